@@ -371,6 +371,67 @@ int yamd_c3_fused(int cin, int ch, int cout, int act, const void *x, int x_cstri
                   const float *bias_packed, int shortcut, void *y, int y_cstride, int batch, int h, int w, void *stream);
 
 /* ----------------------------------------------------------------------------------------
+ * Token operators: the layers of a token mixing block over feature maps, forward and backward.  A map's NHWC pixels are
+ * its tokens, so the tensors of the conv graph are read where they are.  No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------- */
+#define YAMD_F32 0
+#define YAMD_BF16 1
+
+/* Layer norm over the c channels of each row (c <= 16384): y = (x - mean) / sqrt(var + eps) * weight + bias.
+ * Rows of `dtype` x_stride elements apart; weight and bias (NULL = 1 and 0) of param_dtype.  mean and rstd (rows floats
+ * each, both or neither) are what the backward pass needs.  y may be x.
+ * Backward: dx (NULL = not wanted) of dtype; dweight and dbias (NULL = not wanted) of param_dtype, c elements, the sums over
+ * all rows; the workspace is needed for these two.  rows == 0 gives zero dweight and dbias. */
+int yamd_layer_norm(const void *x, long long x_stride, const void *weight, const void *bias, int param_dtype, float eps, void *y,
+                    long long y_stride, float *mean, float *rstd, long long rows, int c, int dtype, void *stream);
+size_t yamd_layer_norm_backward_workspace_bytes(long long rows, int c);
+int yamd_layer_norm_backward(const void *dy, long long dy_stride, const void *x, long long x_stride, const void *weight, int param_dtype,
+                             const float *mean, const float *rstd, void *dx, long long dx_stride, void *dweight, void *dbias,
+                             long long rows, int c, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* bf16 tokens of several heads: channel c of head h of token t of image b is data[b*batch_stride + t*token_stride +
+ * h*head_stride + c].  data is 16-byte aligned, strides are multiples of 8. */
+typedef struct yamd_tokens {
+    void *data;
+    long long batch_stride, token_stride, head_stride;
+} yamd_tokens;
+
+typedef struct yamd_attention_desc {
+    int32_t batch, heads, kv_heads;     /* heads % kv_heads == 0: consecutive heads share a key / value head */
+    int32_t head_dim;                   /* multiple of 8, at most 128 */
+    int32_t q_len, k_len;
+    int32_t map_h, map_w;               /* with a bias: q_len == k_len == map_h * map_w, map_w <= 768 unless map_h == 1 */
+    float scale;                        /* > 0 */
+} yamd_attention_desc;
+
+/* o = softmax(scale q k^T + bias) v for each image and head.
+ *   key_mask  (batch rows of k_len bytes, mask_stride apart; NULL = all): keys with 0 are not attended, and what k and v hold
+ *             there does not matter.  A query that is left without keys gets zeros.
+ *   bias      (heads rows of (2 map_h - 1)(2 map_w - 1) floats; NULL = none): added to the score of a query at (y, x) and a
+ *             key at (y', x') from [(y - y' + map_h - 1)(2 map_w - 1) + x - x' + map_w - 1].
+ *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
+ * The workspace (16-byte aligned; 0 bytes for most shapes) holds parts of o where the keys are split over workgroups. */
+size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biased);
+int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
+                   const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, float *lse,
+                   void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients of the above from o, lse and d_o; the probabilities are computed again.  dbias: one float per head and distance
+ * (given exactly when bias is).  Every sum is taken in a fixed order: equal inputs give equal bits. */
+size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *desc, int biased);
+int yamd_attention_backward(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
+                            const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, const float *lse,
+                            const yamd_tokens *d_o, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv, float *dbias,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
+/* A position bias learned by buckets of distance: bias[head][i] = table[bucket_of[i]][head] for n_distances distances (a
+ * bucket outside the table reads as NaN), and the gradient of the table, dtable[b][head] = sum of dbias[head][order[k]] over
+ * start[b] <= k < start[b + 1].  `order` lists the distances by bucket, `start` has n_buckets + 1 entries. */
+int yamd_relative_bias(const void *table, int table_dtype, const int32_t *bucket_of, int n_distances, int heads, int n_buckets, float *bias,
+                       void *stream);
+int yamd_relative_bias_backward(const float *dbias, const int32_t *order, const int32_t *start, int n_distances, int heads, int n_buckets,
+                                void *dtable, int table_dtype, void *stream);
+
+/* ----------------------------------------------------------------------------------------
  * A model's whole conv graph as one call.  Replaces `out5, out4, out3 = self.body_net(images)`, the module-by-module
  * forward of the backbone + neck + head convs (yolov5/YoloV5.py:54 and :79 over yolov5/YoloV5Body.py:159-187,
  * :223-260; the same statement in every other model class), for callers that do not want one foreign call per layer.

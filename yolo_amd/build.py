@@ -32,11 +32,17 @@ SOURCES = [
     ("yamd_bneck.hip", []),
     ("yamd_c3.hip", []),
     ("yamd_microbench.hip", []),
+    ("yamd_layer_norm.hip", []),
+    ("yamd_attention.hip", []),
+    ("yamd_attention_backward.hip", []),
+    ("yamd_relative_bias.hip", []),
     ("yamd_plan.hip", []),
 ]
-COMMON = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Wall", "-Wno-unused-function"]
+# (no packed float32 instructions: the feature is switched off for the device; the host pass does not know it and says so)
+COMMON = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Wall", "-Wno-unused-function",
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HEADERS = [os.path.join(CSRC, "yamd_common.h"), os.path.join(CSRC, "yamd_conv_kernel.h"),
-           os.path.join(CSRC, "yamd_conv_variants.inc"),
+           os.path.join(CSRC, "yamd_conv_variants.inc"), os.path.join(CSRC, "yamd_attention.h"),
            os.path.join(HERE, "..", "include", "yolo_amd.h")]
 
 

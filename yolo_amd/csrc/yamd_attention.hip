@@ -1,0 +1,370 @@
+// Attention over tokens, forward: o = softmax(scale q k^T + bias) v, bf16 operands, float32 statistics and sums.
+//
+// A wave owns 32 query rows and keeps them in registers as the B operand; a workgroup of four waves walks the keys in tiles
+// of 64 that pass through LDS (two buffers, the next tile's loads in flight under the current one's arithmetic).  The
+// products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane then owns one query, its running maximum, sum and
+// rescaling are scalars of the lane, one exchange between the two halves of the wave completes a maximum, and the
+// probabilities are the second product's B operand in the registers where they were computed (yamd_attention.h).
+// Probabilities are rounded to bf16 for the second product only (their sum is taken before, in float32): the error of o is
+// at most 2^-8 of the weighted mean of |v|, below the rounding of o itself in all but contrived cases.
+//
+// Few query rows: heads that share keys are packed into one tile of rows (row = head in group * q_len + query), and the
+// keys are split over workgroups whose float32 parts a second kernel joins.
+#include "yamd_attention.h"
+
+#include <cmath>
+
+namespace yamd {
+
+struct AttnFwdArgs {
+    AttnView q, k, v;
+    __bf16 *o;
+    long long o_sb, o_st, o_sh;
+    float *lse;                    // [batch][heads][q_len], natural logarithm, or null
+    const uint8_t *mask;           // [batch][k_len], 0 = not attended, or null
+    long long mask_sb;
+    const float *bias;             // [heads][(2 h - 1)(2 w - 1)]
+    int n_off, coord_last, map_w;
+    int batch, q_len, k_len, d, heads, kv_heads, group;
+    int packed, rows, q_tiles, grid_heads, splits, tiles_per_split, total;
+    float scale;
+    float *part_o, *part_ml;       // [split][batch heads][q_len][D] and [...][2] when splits > 1
+};
+
+template <int D>
+struct FwdLds {
+    static constexpr int K = kTile * kRow<D>, BUF = 2 * K, BYTES = 2 * BUF + 2 * kTile * 4;
+};
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
+{
+    using L = FwdLds<D>;
+    constexpr int RB = kRow<D>, NKS = D / 16, NB = D / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *coords = (int *)(smem + 2 * L::BUF);            // a(key) of the tile's rows, two buffers
+
+    int item = work_item();
+    if (item >= a.total) return;
+    const int split = item % a.splits;
+    item /= a.splits;
+    const int q_tile = item % a.q_tiles;
+    item /= a.q_tiles;
+    const int gh = item % a.grid_heads, b = item / a.grid_heads;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c32 = lane & 31, half = lane >> 5;
+    const int row0 = q_tile * kBlockRows + wave * 32;
+    const int row = row0 + c32 < a.rows ? row0 + c32 : a.rows - 1;     // lanes beyond the rows repeat the last one
+    const int in_group = a.packed ? row / a.q_len : 0;
+    const int i = row - in_group * a.q_len;
+    const int head = a.packed ? gh * a.group + in_group : gh;
+    const int kv_head = a.packed ? gh : gh / a.group;
+
+    bf16x8 qf[NKS];
+    {
+        const __bf16 *qp = a.q.p + b * a.q.sb + (long long)i * a.q.st + head * a.q.sh;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            const int c = 16 * ks + 8 * half;
+            if (c < a.d) qf[ks] = *(const bf16x8 *)(qp + c);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[ks][e] = (__bf16)0.0f;
+        }
+    }
+    const __bf16 *kp = a.k.p + b * a.k.sb + kv_head * a.k.sh, *vp = a.v.p + b * a.v.sb + kv_head * a.v.sh;
+    const uint8_t *mp = a.mask ? a.mask + b * a.mask_sb : nullptr;
+    const float *bp = BIAS ? a.bias + (long long)head * a.n_off + a.coord_last + map_coord(i, a.map_w) : nullptr;
+
+    f32x16 acc[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[n] = zero16();
+    float m = -INFINITY, l = 0.0f;                       // running maximum and this half's sum, in units of log 2
+    const float c2 = a.scale * kLog2e;
+
+    const int t0 = split * a.tiles_per_split, n_tiles = (a.k_len + kTile - 1) / kTile;
+    const int t1 = t0 + a.tiles_per_split < n_tiles ? t0 + a.tiles_per_split : n_tiles;
+    TilePieces<D> kn, vn;
+    bool valid_n = false;
+    auto fetch = [&](int t) {
+        const int first = t * kTile;
+        kn.load(kp, a.k.st, first, a.k_len, a.d);
+        vn.load(vp, a.v.st, first, a.k_len, a.d);
+        valid_n = first + lane < a.k_len && (!mp || mp[first + lane] != 0);
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::K;
+        int *const ct = coords + (t & 1) * kTile;
+        const unsigned long long keep = __ballot(valid_n);
+        kn.store(kt, RB, keep);
+        vn.store(vt, RB, keep);
+        if (BIAS && tid < kTile) {
+            const int key = t * kTile + tid;
+            ct[tid] = map_coord(key < a.k_len ? key : a.k_len - 1, a.map_w);
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        if (keep == 0 || row0 >= a.rows) continue;       // a tile without keys, a wave without rows
+
+        f32x16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = zero16();
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) s[u] = mfma(rows_operand(kt, RB, 32 * u, ks, lane), qf[ks], s[u]);
+        }
+        if constexpr (BIAS) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = s[u][r] * c2 + bp[-ct[32 * u + acc_row(r, half)]] * kLog2e;
+        }
+        if (keep != ~0ull) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!((keep >> (32 * u + acc_row(r, half))) & 1)) s[u][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+        top = with_other_half(top, [](float x, float y) { return fmaxf(x, y); });
+        if constexpr (!BIAS) top *= c2;
+        if (__any(top > m)) {
+            const float m_new = fmaxf(m, top);
+            const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+            m = m_new;
+            l *= f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[n][r] *= f;
+        }
+        const float sub = m == -INFINITY ? 0.0f : m;     // rows without a key so far: every term below is exp2(-inf) = 0
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(BIAS ? s[u][r] - sub : __builtin_fmaf(s[u][r], c2, -sub));
+                l += s[u][r];
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bf16x8 pf = acc_operand(s[u >> 1], u & 1);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) acc[n] = mfma(transposed_operand(vt, RB, 16 * u, 32 * n, lane), pf, acc[n]);
+        }
+    }
+    l = with_other_half(l, [](float x, float y) { return x + y; });
+    if (row0 + c32 >= a.rows) return;
+    if (a.splits > 1) {
+        const long long at = (((long long)split * a.batch + b) * a.heads + head) * a.q_len + i;
+        if (half == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m, l);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 o = {acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2], acc[n][4 * g + 3]};
+                *(f32x4 *)(a.part_o + at * D + 32 * n + 8 * g + 4 * half) = o;
+            }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    __bf16 *op = a.o + b * a.o_sb + (long long)i * a.o_st + head * a.o_sh;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * n + 8 * g + 4 * half;
+            if (c < a.d) {
+                bf16x4 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (__bf16)(acc[n][4 * g + e] * inv);
+                *(bf16x4 *)(op + c) = o;
+            }
+        }
+    if (a.lse && half == 0)
+        a.lse[((long long)b * a.heads + head) * a.q_len + i] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
+}
+
+// joins the parts of a split key axis: one thread per (row, 4 channels)
+template <int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long long rows)
+{
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long at = id / (D / 4);
+    const int c = (int)(id % (D / 4)) * 4;
+    if (at >= rows) return;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + at)]);
+    const float sub = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 ml = *(const float2 *)(a.part_ml + 2 * (s * rows + at));
+        const float f = __builtin_amdgcn_exp2f(ml.x - sub);
+        l += ml.y * f;
+        const f32x4 p = *(const f32x4 *)(a.part_o + (s * rows + at) * D + c);
+        o += p * f;
+    }
+    const int i = (int)(at % a.q_len);
+    const long long bh = at / a.q_len;
+    const int head = (int)(bh % a.heads);
+    const long long b = bh / a.heads;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (c < a.d) {
+        bf16x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (__bf16)(o[e] * inv);
+        *(bf16x4 *)(a.o + b * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
+    }
+    if (a.lse && c == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+int check_attention(const yamd_attention_desc *d, const uint8_t *key_mask, long long mask_stride, const float *bias)
+{
+    YAMD_REQUIRE(d, "attention: null descriptor");
+    YAMD_REQUIRE(d->batch > 0 && d->q_len > 0 && d->k_len > 0 && d->heads > 0 && d->kv_heads > 0,
+                 "attention: bad shape batch=%d q_len=%d k_len=%d heads=%d kv_heads=%d", d->batch, d->q_len, d->k_len, d->heads, d->kv_heads);
+    YAMD_REQUIRE(d->heads % d->kv_heads == 0, "attention: %d heads do not share %d key heads evenly", d->heads, d->kv_heads);
+    YAMD_REQUIRE(d->head_dim >= 8 && d->head_dim <= 128 && d->head_dim % 8 == 0,
+                 "attention: head_dim must be a multiple of 8 up to 128 (got %d)", d->head_dim);
+    YAMD_REQUIRE(d->q_len <= (1 << 24) && d->k_len <= (1 << 24), "attention: more than 2^24 tokens (q %d, k %d)", d->q_len, d->k_len);
+    YAMD_REQUIRE((long long)d->batch * d->heads <= (1 << 20), "attention: batch * heads = %lld above 2^20", (long long)d->batch * d->heads);
+    YAMD_REQUIRE(d->scale > 0.0f && d->scale < INFINITY, "attention: scale must be positive and finite (got %g)", (double)d->scale);
+    YAMD_REQUIRE(!key_mask || d->batch == 1 || mask_stride >= d->k_len, "attention: mask stride smaller than k_len");
+    if (bias) {
+        YAMD_REQUIRE(d->map_h > 0 && d->map_w > 0 && d->q_len == d->k_len && (long long)d->map_h * d->map_w == d->q_len,
+                     "attention: a position bias needs q_len == k_len == map_h * map_w (got %d, %d, %d x %d)", d->q_len, d->k_len, d->map_h,
+                     d->map_w);
+        YAMD_REQUIRE(d->map_h == 1 || d->map_w <= 768, "attention: a map of several rows is at most 768 wide (got %d x %d)", d->map_h, d->map_w);
+    }
+    return YAMD_OK;
+}
+
+int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, int heads, const char *name)
+{
+    YAMD_REQUIRE(t && t->data, "attention: %s is null", name);
+    YAMD_REQUIRE(((uintptr_t)t->data & 15) == 0, "attention: %s is not 16-byte aligned", name);
+    YAMD_REQUIRE((d->batch == 1 || (t->batch_stride % 8 == 0 && t->batch_stride >= 0)) && (len == 1 || (t->token_stride % 8 == 0 && t->token_stride > 0)) &&
+                     (heads == 1 || (t->head_stride % 8 == 0 && t->head_stride > 0)),
+                 "attention: strides of %s must be positive multiples of 8 elements", name);
+    return YAMD_OK;
+}
+
+int attention_splits(long long workgroups, int tiles, int min_tiles)
+{
+    // up to about 4 workgroups for each of the 256 CUs, and at least `min_tiles` tiles for each part
+    const long long want = 1024 / workgroups, most = tiles / min_tiles;
+    const long long n = want < most ? want : most;
+    return n < 1 ? 1 : (int)n;
+}
+
+namespace {
+
+struct FwdPlan {
+    int packed, rows, q_tiles, grid_heads, splits, tiles_per_split, dpad;
+    long long total;
+    size_t workspace;
+};
+
+FwdPlan plan_forward(const yamd_attention_desc *d, bool biased)
+{
+    FwdPlan p = {};
+    const int group = d->heads / d->kv_heads;
+    p.dpad = padded_head_dim(d->head_dim);
+    // packing shares a tile of keys among the group's heads; with a full tile of queries per head there is nothing to gain
+    p.packed = !biased && group > 1 && d->q_len <= kBlockRows / 2;
+    p.rows = p.packed ? d->q_len * group : d->q_len;
+    p.grid_heads = p.packed ? d->kv_heads : d->heads;
+    p.q_tiles = ceil_div(p.rows, kBlockRows);
+    const int n_tiles = ceil_div(d->k_len, kTile);
+    const long long wgs = (long long)d->batch * p.grid_heads * p.q_tiles;
+    const int splits = wgs >= 512 ? 1 : attention_splits(wgs, n_tiles, 4);
+    p.tiles_per_split = ceil_div(n_tiles, splits);
+    p.splits = ceil_div(n_tiles, p.tiles_per_split);
+    p.total = wgs * p.splits;
+    if (p.splits > 1) p.workspace = (size_t)p.splits * d->batch * d->heads * d->q_len * (p.dpad + 2) * sizeof(float);
+    return p;
+}
+
+template <int D, bool BIAS>
+int launch_forward(const AttnFwdArgs &a, long long rows, hipStream_t st)
+{
+    using Attr = KernelAttr<&attention_kernel<D, BIAS>, FwdLds<D>::BYTES>;
+    const int rc = Attr::ensure();
+    if (rc != YAMD_OK) return rc;
+    hipLaunchKernelGGL((attention_kernel<D, BIAS>), dim3(work_grid(a.total)), dim3(256), FwdLds<D>::BYTES, st, a);
+    YAMD_LAUNCH_CHECK();
+    if (a.splits > 1) {
+        hipLaunchKernelGGL((attention_join_kernel<D>), dim3(ceil_div(rows * (D / 4), 256)), dim3(256), 0, st, a, rows);
+        YAMD_LAUNCH_CHECK();
+    }
+    return YAMD_OK;
+}
+
+}  // namespace
+}  // namespace yamd
+
+using namespace yamd;
+
+extern "C" size_t yamd_attention_workspace_bytes(const yamd_attention_desc *d, int biased)
+{
+    if (check_attention(d, nullptr, 0, nullptr) != YAMD_OK) return 0;
+    return plan_forward(d, biased != 0).workspace;
+}
+
+extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
+                              const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, float *lse,
+                              void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_attention(d, key_mask, mask_stride, bias);
+    if (rc == YAMD_OK) rc = check_tokens(d, q, d->q_len, d->heads, "q");
+    if (rc == YAMD_OK) rc = check_tokens(d, k, d->k_len, d->kv_heads, "k");
+    if (rc == YAMD_OK) rc = check_tokens(d, v, d->k_len, d->kv_heads, "v");
+    if (rc == YAMD_OK) rc = check_tokens(d, o, d->q_len, d->heads, "o");
+    if (rc != YAMD_OK) return rc;
+    const FwdPlan p = plan_forward(d, bias != nullptr);
+    YAMD_REQUIRE(p.total <= (1ll << 30), "attention: %lld workgroups", p.total);
+    if (p.workspace && (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15))) {
+        set_error("attention: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace ? workspace_bytes : (size_t)0, p.workspace);
+        return YAMD_ENOSPC;
+    }
+    AttnFwdArgs a = {};
+    a.q = view_of(q); a.k = view_of(k); a.v = view_of(v);
+    a.o = (__bf16 *)o->data; a.o_sb = o->batch_stride; a.o_st = o->token_stride; a.o_sh = o->head_stride;
+    a.lse = lse; a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
+    if (bias) {
+        a.map_w = d->map_w;
+        a.coord_last = map_coord(d->k_len - 1, d->map_w);
+        a.n_off = 2 * a.coord_last + 1;
+    }
+    a.batch = d->batch; a.q_len = d->q_len; a.k_len = d->k_len; a.d = d->head_dim; a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads;
+    a.packed = p.packed; a.rows = p.rows; a.q_tiles = p.q_tiles; a.grid_heads = p.grid_heads; a.splits = p.splits;
+    a.tiles_per_split = p.tiles_per_split; a.total = (int)p.total; a.scale = d->scale;
+    const long long rows = (long long)d->batch * d->heads * d->q_len;
+    if (p.splits > 1) {
+        a.part_o = (float *)workspace;
+        a.part_ml = a.part_o + (size_t)p.splits * rows * p.dpad;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    if (bias) {
+        switch (p.dpad) {
+        case 32: return launch_forward<32, true>(a, rows, st);
+        case 64: return launch_forward<64, true>(a, rows, st);
+        case 96: return launch_forward<96, true>(a, rows, st);
+        default: return launch_forward<128, true>(a, rows, st);
+        }
+    }
+    switch (p.dpad) {
+    case 32: return launch_forward<32, false>(a, rows, st);
+    case 64: return launch_forward<64, false>(a, rows, st);
+    case 96: return launch_forward<96, false>(a, rows, st);
+    default: return launch_forward<128, false>(a, rows, st);
+    }
+}

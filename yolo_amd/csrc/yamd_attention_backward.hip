@@ -1,0 +1,596 @@
+// Attention over tokens, backward.  The probabilities are computed again from q, k and the forward pass's logarithm of the
+// sums, so nothing of size q_len x k_len is kept:
+//   P = exp(scale q k^T + bias - lse),  dP = do v^T,  D = rowsum(do o),  dS = P (dP - D)
+//   dv = P^T do,  dk = scale dS^T q,  dq = scale dS k,  d bias[distance] = sum of dS over the pairs at that distance
+//
+// Two kernels share the work so that every sum has one owner and a fixed order (no atomics on gradients, equal bits on every
+// run): one owns keys and walks the queries of all heads that share them (dk, dv), one owns queries and walks the keys (dq,
+// bias).  That costs 7 products instead of 5; float32 atomics on dq would instead cost its size once per key block.
+// Both take the products so that P and dS come out as the B operand of the product that follows (yamd_attention.h); P and
+// dS are rounded to bf16 there, their use in the sums before (bias) stays in float32.
+#include "yamd_attention.h"
+
+#include <cmath>
+
+namespace yamd {
+
+struct AttnBwdArgs {
+    AttnView q, k, v, o, go;
+    const float *lse;
+    float *delta;                  // [batch][heads][q_len]: D
+    const uint8_t *mask;
+    long long mask_sb;
+    const float *bias;
+    int n_off, coord_last, map_w;
+    int batch, q_len, k_len, d, heads, kv_heads, group;
+    float scale;
+    // one of the two owning kernels
+    int tiles, splits, loop_per_split, total;
+    __bf16 *out0, *out1;           // dk, dv / dq
+    long long o0_sb, o0_st, o0_sh, o1_sb, o1_st, o1_sh;
+    float *part0, *part1;          // float32 parts [split][batch * heads][len][D] when splits > 1
+    float *part_bias;              // [batch * heads * tiles][part_len]: sums by distance of one workgroup
+    int ring, part_len;
+};
+
+// D = rowsum(do o): 16 lanes per row, 8 channels each.  A row without keys (lse = -inf) has no gradient whatever do holds.
+__global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
+{
+    const long long rows = (long long)a.batch * a.heads * a.q_len;
+    const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int c = (threadIdx.x & 15) * 8;
+    float s = 0.0f;
+    if (at < rows) {
+        // rows in the order (batch, token, head), which is the order in memory of the usual layout
+        const int head = (int)(at % a.heads), i = (int)(at / a.heads % a.q_len);
+        const long long b = at / a.heads / a.q_len;
+        if (c < a.d) {
+            const bf16x8 o = *(const bf16x8 *)(a.o.p + b * a.o.sb + (long long)i * a.o.st + head * a.o.sh + c);
+            const bf16x8 g = *(const bf16x8 *)(a.go.p + b * a.go.sb + (long long)i * a.go.st + head * a.go.sh + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += (float)o[e] * (float)g[e];
+        }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        const long long w = (b * a.heads + head) * a.q_len + i;
+        if ((threadIdx.x & 15) == 0) a.delta[w] = a.lse[w] == -INFINITY ? 0.0f : s;
+    }
+}
+
+// ---- dk, dv ------------------------------------------------------------------------------------------------------------
+// A wave owns 32 keys (the result's columns); tiles of 64 queries pass through LDS.  S = Q K^T and dP = dO V^T read the
+// tile's rows, dV^T += dO^T P and dK^T += Q^T dS read it transposed.
+template <int D>
+struct KvLds {
+    static constexpr int T = kTile * kRow<D>, BUF = 2 * T + 3 * kTile * 4, BYTES = 2 * BUF;
+};
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
+{
+    using L = KvLds<D>;
+    constexpr int RB = kRow<D>, NKS = D / 16, NB = D / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+
+    int item = work_item();
+    if (item >= a.total) return;
+    const int split = item % a.splits;
+    item /= a.splits;
+    const int tile = item % a.tiles;
+    item /= a.tiles;
+    const int kv_head = item % a.kv_heads, b = item / a.kv_heads;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c32 = lane & 31, half = lane >> 5;
+    const int key0 = tile * kBlockRows + wave * 32;
+    const int key = key0 + c32 < a.k_len ? key0 + c32 : a.k_len - 1;
+    const bool valid = key0 + c32 < a.k_len && (!a.mask || a.mask[b * a.mask_sb + key] != 0);
+    const bool busy = __any(valid);
+
+    bf16x8 kf[NKS], vf[NKS];
+    {
+        const __bf16 *kp = a.k.p + b * a.k.sb + (long long)key * a.k.st + kv_head * a.k.sh;
+        const __bf16 *vp = a.v.p + b * a.v.sb + (long long)key * a.v.st + kv_head * a.v.sh;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            const int c = 16 * ks + 8 * half;
+            if (valid && c < a.d) {
+                kf[ks] = *(const bf16x8 *)(kp + c);
+                vf[ks] = *(const bf16x8 *)(vp + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) kf[ks][e] = vf[ks][e] = (__bf16)0.0f;
+            }
+        }
+    }
+    const int ck = BIAS ? a.coord_last - map_coord(key, a.map_w) : 0;
+
+    f32x16 dk[NB], dv[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) dk[n] = zero16(), dv[n] = zero16();
+    const float c2 = a.scale * kLog2e;
+
+    // the loop runs over (head of the group, tile of queries)
+    const int q_tiles = (a.q_len + kTile - 1) / kTile, loop = a.group * q_tiles;
+    const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < loop ? t0 + a.loop_per_split : loop;
+    TilePieces<D> qn, gn;
+    float lse_n = 0.0f, delta_n = 0.0f;
+    auto fetch = [&](int t) {
+        const int head = kv_head * a.group + t / q_tiles, first = t % q_tiles * kTile;
+        qn.load(a.q.p + b * a.q.sb + head * a.q.sh, a.q.st, first, a.q_len, a.d);
+        gn.load(a.go.p + b * a.go.sb + head * a.go.sh, a.go.st, first, a.q_len, a.d);
+        // rows beyond the queries, and rows without keys, get an infinite sum: their probabilities are exp2(-inf) = 0
+        lse_n = INFINITY;
+        delta_n = 0.0f;
+        if (first + lane < a.q_len) {
+            const long long w = ((long long)b * a.heads + head) * a.q_len + first + lane;
+            lse_n = a.lse[w] == -INFINITY ? INFINITY : a.lse[w];
+            delta_n = a.delta[w];
+        }
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        char *const qt = smem + (t & 1) * L::BUF, *const gt = qt + L::T;
+        float *const lse2 = (float *)(gt + L::T), *const delta = lse2 + kTile;
+        int *const coord = (int *)(delta + kTile);
+        const unsigned long long keep = __ballot(lse_n != INFINITY);
+        qn.store(qt, RB, keep);                        // a row without keys gives no gradient whatever q and do hold
+        gn.store(gt, RB, keep);
+        if (tid < kTile) {
+            lse2[tid] = lse_n * kLog2e;
+            delta[tid] = delta_n;
+            if (BIAS) {
+                const int i = t % q_tiles * kTile + tid;
+                coord[tid] = map_coord(i < a.q_len ? i : a.q_len - 1, a.map_w);
+            }
+        }
+        const float *bp = BIAS ? a.bias + (long long)(kv_head * a.group + t / q_tiles) * a.n_off + ck : nullptr;
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        if (!busy) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f32x16 s = zero16(), g = zero16();
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) s = mfma(rows_operand(qt, RB, 32 * u, ks, lane), kf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) g = mfma(rows_operand(gt, RB, 32 * u, ks, lane), vf[ks], g);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int at = 32 * u + acc_row(r, half);
+                const float x = BIAS ? bp[coord[at]] * kLog2e - lse2[at] : -lse2[at];
+                const float p = valid ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, x)) : 0.0f;
+                s[r] = p;
+                g[r] = p * (g[r] - delta[at]);
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const bf16x8 pf = acc_operand(s, w), sf = acc_operand(g, w);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    dv[n] = mfma(transposed_operand(gt, RB, 32 * u + 16 * w, 32 * n, lane), pf, dv[n]);
+                    dk[n] = mfma(transposed_operand(qt, RB, 32 * u + 16 * w, 32 * n, lane), sf, dk[n]);
+                }
+            }
+        }
+    }
+    if (key0 + c32 >= a.k_len) return;
+    if (!valid) {                                      // a masked key has no gradient whatever the queries hold
+#pragma unroll
+        for (int n = 0; n < NB; ++n) dk[n] = zero16(), dv[n] = zero16();
+    }
+    if (a.splits > 1) {
+        const long long at = ((((long long)split * a.batch + b) * a.kv_heads + kv_head) * a.k_len + key) * D;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * n + 8 * g + 4 * half;
+                *(f32x4 *)(a.part0 + at + c) = f32x4{dk[n][4 * g], dk[n][4 * g + 1], dk[n][4 * g + 2], dk[n][4 * g + 3]};
+                *(f32x4 *)(a.part1 + at + c) = f32x4{dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]};
+            }
+        return;
+    }
+    __bf16 *kp = a.out0 + b * a.o0_sb + (long long)key * a.o0_st + kv_head * a.o0_sh;
+    __bf16 *vp = a.out1 + b * a.o1_sb + (long long)key * a.o1_st + kv_head * a.o1_sh;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * n + 8 * g + 4 * half;
+            if (c < a.d) {
+                bf16x4 x, y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (__bf16)(dk[n][4 * g + e] * a.scale), y[e] = (__bf16)dv[n][4 * g + e];
+                *(bf16x4 *)(kp + c) = x;
+                *(bf16x4 *)(vp + c) = y;
+            }
+        }
+}
+
+// ---- dq, bias ----------------------------------------------------------------------------------------------------------
+// A wave owns 32 queries (the result's columns); tiles of 64 keys pass through LDS.  S^T = K Q^T and dP^T = V dO^T read the
+// tile's rows, dQ^T += K^T dS^T reads the keys transposed.
+//
+// The bias gradient is summed by distance.  For one key, the 32 queries of a half wave lie at 32 different distances, so
+// the wave adds its dS values into a ring of float32 sums in LDS of its own without two lanes of a half meeting.  As the
+// keys advance the distances fall: those above a(last query) - a(first key of the next tile) are final, and after each
+// tile the workgroup adds the four waves' rings in a fixed order for them, writes them to its row of the workspace and
+// clears them.  The ring must hold the distances of two tiles (one being added to while the other is written out):
+// 2 * 127 + 1 positions, and where a map has several rows 127 + 127 + 2 w more.
+template <int D>
+struct QLds {
+    static constexpr int T = kTile * kRow<D>, BUF = 2 * T + kTile * 4, BYTES = 2 * BUF;
+};
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
+{
+    using L = QLds<D>;
+    constexpr int RB = kRow<D>, NKS = D / 16, NB = D / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float *const rings = (float *)(smem + L::BYTES);
+
+    int item = work_item();
+    if (item >= a.total) return;
+    const int wg = item;
+    const int split = item % a.splits;
+    item /= a.splits;
+    const int tile = item % a.tiles;
+    item /= a.tiles;
+    const int head = item % a.heads, b = item / a.heads, kv_head = head / a.group;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c32 = lane & 31, half = lane >> 5;
+    const int row0 = tile * kBlockRows + wave * 32;
+    const int i = row0 + c32 < a.q_len ? row0 + c32 : a.q_len - 1;
+    const long long stat = ((long long)b * a.heads + head) * a.q_len + i;
+    const float lse = a.lse[stat];
+    const bool valid = row0 + c32 < a.q_len && lse != -INFINITY;
+    const float lse2 = valid ? lse * kLog2e : INFINITY, delta = a.delta[stat];
+    const bool busy = __any(valid);
+
+    bf16x8 qf[NKS], gf[NKS];
+    {
+        const __bf16 *qp = a.q.p + b * a.q.sb + (long long)i * a.q.st + head * a.q.sh;
+        const __bf16 *gp = a.go.p + b * a.go.sb + (long long)i * a.go.st + head * a.go.sh;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            const int c = 16 * ks + 8 * half;
+            if (valid && c < a.d) {
+                qf[ks] = *(const bf16x8 *)(qp + c);
+                gf[ks] = *(const bf16x8 *)(gp + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[ks][e] = gf[ks][e] = (__bf16)0.0f;
+            }
+        }
+    }
+    const __bf16 *kp = a.k.p + b * a.k.sb + kv_head * a.k.sh, *vp = a.v.p + b * a.v.sb + kv_head * a.v.sh;
+    const uint8_t *mp = a.mask ? a.mask + b * a.mask_sb : nullptr;
+
+    // distance index of (query, key) = cq - a(key); of the workgroup's rows the first and last
+    int cq = 0, c_first = 0, c_last = 0, high = 0;
+    const float *bp = nullptr;
+    float *ring = nullptr;
+    if constexpr (BIAS) {
+        const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
+        cq = a.coord_last + map_coord(i, a.map_w);
+        c_first = a.coord_last + map_coord(tile * kBlockRows, a.map_w);
+        c_last = a.coord_last + map_coord(last, a.map_w);
+        high = c_last + 1;                             // distances from here on are written out (a(0) = 0)
+        bp = a.bias + (long long)head * a.n_off + cq;
+        ring = rings + wave * a.ring;
+        for (int e = tid; e < 4 * a.ring; e += 256) rings[e] = 0.0f;
+    }
+
+    f32x16 dq[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) dq[n] = zero16();
+    const float c2 = a.scale * kLog2e;
+
+    const int n_tiles = (a.k_len + kTile - 1) / kTile;
+    const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < n_tiles ? t0 + a.loop_per_split : n_tiles;
+    TilePieces<D> kn, vn;
+    bool valid_n = false;
+    auto fetch = [&](int t) {
+        const int first = t * kTile;
+        kn.load(kp, a.k.st, first, a.k_len, a.d);
+        vn.load(vp, a.v.st, first, a.k_len, a.d);
+        valid_n = first + lane < a.k_len && (!mp || mp[first + lane] != 0);
+    };
+    // writes the sums of the distances [low, high) out and clears them
+    auto flush = [&](int low) {
+        float *out = a.part_bias + (long long)wg * a.part_len;
+        const int base = c_first - a.coord_last;       // the smallest distance of the workgroup: first query, last key
+        for (int e = low + tid; e < high; e += 256) {
+            const int at = e & (a.ring - 1);
+            float s = rings[at];
+            rings[at] = 0.0f;
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+                s += rings[w * a.ring + at];
+                rings[w * a.ring + at] = 0.0f;
+            }
+            out[e - base] = s;
+        }
+        high = low;
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::T;
+        int *const ct = (int *)(vt + L::T);
+        const unsigned long long keep = __ballot(valid_n);
+        kn.store(kt, RB, keep);
+        vn.store(vt, RB, keep);
+        if (BIAS && tid < kTile) {
+            const int key = t * kTile + tid;
+            ct[tid] = map_coord(key < a.k_len ? key : a.k_len - 1, a.map_w);
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        if constexpr (BIAS) flush(c_last - map_coord(t * kTile, a.map_w) + 1);   // what the tiles before this one left final
+        if (!busy || keep == 0) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f32x16 s = zero16(), g = zero16();
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) s = mfma(rows_operand(kt, RB, 32 * u, ks, lane), qf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) g = mfma(rows_operand(vt, RB, 32 * u, ks, lane), gf[ks], g);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int at = 32 * u + acc_row(r, half);
+                int ca = 0;
+                float x = -lse2;
+                if constexpr (BIAS) {
+                    ca = ct[at];
+                    x += bp[-ca] * kLog2e;
+                }
+                const float p = (keep >> at) & 1 ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, x)) : 0.0f;
+                g[r] = p * (g[r] - delta);
+                if constexpr (BIAS) {
+                    // lanes without a query repeat the last one with dS = 0
+                    __hip_atomic_fetch_add(ring + ((cq - ca) & (a.ring - 1)), g[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const bf16x8 sf = acc_operand(g, w);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) dq[n] = mfma(transposed_operand(kt, RB, 32 * u + 16 * w, 32 * n, lane), sf, dq[n]);
+            }
+        }
+    }
+    if constexpr (BIAS) {
+        __syncthreads();
+        flush(c_first - a.coord_last);
+    }
+    if (row0 + c32 >= a.q_len) return;
+    if (a.splits > 1) {
+        const long long at = ((((long long)split * a.batch + b) * a.heads + head) * a.q_len + i) * D;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(f32x4 *)(a.part0 + at + 32 * n + 8 * g + 4 * half) =
+                    f32x4{dq[n][4 * g], dq[n][4 * g + 1], dq[n][4 * g + 2], dq[n][4 * g + 3]};
+        return;
+    }
+    __bf16 *op = a.out0 + b * a.o0_sb + (long long)i * a.o0_st + head * a.o0_sh;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * n + 8 * g + 4 * half;
+            if (c < a.d) {
+                bf16x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (__bf16)(dq[n][4 * g + e] * a.scale);
+                *(bf16x4 *)(op + c) = x;
+            }
+        }
+}
+
+// adds the workgroups' sums by distance: thread = one distance of one head, workgroups in the order (batch, tile)
+__global__ __launch_bounds__(256) void attention_bias_grad_kernel(AttnBwdArgs a, float *dbias)
+{
+    const int off = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
+    if (off >= a.n_off) return;
+    float s = 0.0f;
+    for (int tile = 0; tile < a.tiles; ++tile) {
+        const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
+        const int base = map_coord(tile * kBlockRows, a.map_w), n = map_coord(last, a.map_w) + a.coord_last - base + 1;
+        if (off < base || off - base >= n) continue;
+        for (int b = 0; b < a.batch; ++b) s += a.part_bias[(((long long)b * a.heads + head) * a.tiles + tile) * a.part_len + off - base];
+    }
+    dbias[(long long)head * a.n_off + off] = s;
+}
+
+struct SumArgs {
+    const float *parts;
+    long long rows;                // batch * heads * len
+    int splits, heads, len, d, dpad;
+    float scale;
+    __bf16 *out;
+    long long sb, st, sh;
+};
+
+__global__ __launch_bounds__(256) void attention_sum_parts_kernel(SumArgs a)
+{
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int per_row = a.dpad / 4;
+    const long long at = id / per_row;
+    const int c = (int)(id % per_row) * 4;
+    if (at >= a.rows || c >= a.d) return;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < a.splits; ++k) s += *(const f32x4 *)(a.parts + (k * a.rows + at) * a.dpad + c);
+    const int t = (int)(at % a.len), head = (int)(at / a.len % a.heads);
+    const long long b = at / a.len / a.heads;
+    bf16x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (__bf16)(s[e] * a.scale);
+    *(bf16x4 *)(a.out + b * a.sb + (long long)t * a.st + head * a.sh + c) = o;
+}
+
+namespace {
+
+int launch_sum_parts(const AttnBwdArgs &p, const float *parts, int heads, int len, int dpad, float scale, __bf16 *out, long long sb,
+                     long long st, long long sh, hipStream_t stream)
+{
+    SumArgs a = {parts, (long long)p.batch * heads * len, p.splits, heads, len, p.d, dpad, scale, out, sb, st, sh};
+    hipLaunchKernelGGL(attention_sum_parts_kernel, dim3(ceil_div(a.rows * (dpad / 4), 256)), dim3(256), 0, stream, a);
+    YAMD_LAUNCH_CHECK();
+    return YAMD_OK;
+}
+
+struct BwdPlan {
+    int dpad, kv_tiles, kv_splits, kv_loop, q_tiles, q_splits, q_loop, ring, part_len;
+    long long kv_total, q_total;
+    size_t delta, parts, bias, workspace;     // bytes; the parts of dk and dv and those of dq use the same memory in turn
+};
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
+{
+    BwdPlan p = {};
+    p.dpad = padded_head_dim(d->head_dim);
+    const long long bh = (long long)d->batch * d->heads, bk = (long long)d->batch * d->kv_heads;
+    const int kt = ceil_div(d->k_len, kTile), qt = ceil_div(d->q_len, kTile) * (d->heads / d->kv_heads);
+    p.kv_tiles = ceil_div(d->k_len, kBlockRows);
+    p.q_tiles = ceil_div(d->q_len, kBlockRows);
+    const long long kw = bk * p.kv_tiles, qw = bh * p.q_tiles;
+    const int ks = kw >= 512 ? 1 : attention_splits(kw, qt, 4);
+    p.kv_loop = ceil_div(qt, ks);
+    p.kv_splits = ceil_div(qt, p.kv_loop);
+    const int qs = biased || qw >= 512 ? 1 : attention_splits(qw, kt, 4);   // one owner per row of distances
+    p.q_loop = ceil_div(kt, qs);
+    p.q_splits = ceil_div(kt, p.q_loop);
+    p.kv_total = kw * p.kv_splits;
+    p.q_total = qw * p.q_splits;
+    p.delta = up256((size_t)bh * d->q_len * sizeof(float));
+    const size_t pk = p.kv_splits > 1 ? 2 * (size_t)p.kv_splits * bk * d->k_len * p.dpad * sizeof(float) : 0;
+    const size_t pq = p.q_splits > 1 ? (size_t)p.q_splits * bh * d->q_len * p.dpad * sizeof(float) : 0;
+    p.parts = up256(pk > pq ? pk : pq);
+    if (biased) {
+        const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
+        for (p.ring = 256; p.ring < span; p.ring *= 2) {}
+        const int coord_last = map_coord(d->k_len - 1, d->map_w);
+        p.part_len = coord_last + kBlockRows + (d->map_h > 1 ? kBlockRows + w : 0);
+        p.bias = up256((size_t)bh * p.q_tiles * p.part_len * sizeof(float));
+    }
+    p.workspace = p.delta + p.parts + p.bias;
+    return p;
+}
+
+template <int D, bool BIAS>
+int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv, float *dbias,
+                    hipStream_t st)
+{
+    constexpr int kRingBytes = BIAS ? 4 * 2048 * 4 : 0;
+    using KvAttr = KernelAttr<&attention_dkv_kernel<D, BIAS>, KvLds<D>::BYTES>;
+    using QAttr = KernelAttr<&attention_dq_kernel<D, BIAS>, QLds<D>::BYTES + kRingBytes>;
+    int rc = KvAttr::ensure();
+    if (rc == YAMD_OK) rc = QAttr::ensure();
+    if (rc != YAMD_OK) return rc;
+    const long long rows = (long long)a.batch * a.heads * a.q_len;
+    hipLaunchKernelGGL(attention_delta_kernel, dim3(ceil_div(rows, 16)), dim3(256), 0, st, a);
+    YAMD_LAUNCH_CHECK();
+
+    AttnBwdArgs w = a;
+    w.tiles = p.kv_tiles; w.splits = p.kv_splits; w.loop_per_split = p.kv_loop; w.total = (int)p.kv_total;
+    w.out0 = (__bf16 *)dk->data; w.o0_sb = dk->batch_stride; w.o0_st = dk->token_stride; w.o0_sh = dk->head_stride;
+    w.out1 = (__bf16 *)dv->data; w.o1_sb = dv->batch_stride; w.o1_st = dv->token_stride; w.o1_sh = dv->head_stride;
+    const size_t half = (size_t)p.kv_splits * a.batch * a.kv_heads * a.k_len * D;
+    w.part1 = w.part0 + half;
+    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256), KvLds<D>::BYTES, st, w);
+    YAMD_LAUNCH_CHECK();
+    if (w.splits > 1) {
+        rc = launch_sum_parts(w, w.part0, a.kv_heads, a.k_len, D, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh, st);
+        if (rc == YAMD_OK) rc = launch_sum_parts(w, w.part1, a.kv_heads, a.k_len, D, 1.0f, w.out1, w.o1_sb, w.o1_st, w.o1_sh, st);
+        if (rc != YAMD_OK) return rc;
+    }
+
+    w = a;
+    w.tiles = p.q_tiles; w.splits = p.q_splits; w.loop_per_split = p.q_loop; w.total = (int)p.q_total;
+    w.out0 = (__bf16 *)dq->data; w.o0_sb = dq->batch_stride; w.o0_st = dq->token_stride; w.o0_sh = dq->head_stride;
+    hipLaunchKernelGGL((attention_dq_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256),
+                       QLds<D>::BYTES + (BIAS ? 4 * p.ring * (int)sizeof(float) : 0), st, w);
+    YAMD_LAUNCH_CHECK();
+    if (w.splits > 1) {
+        rc = launch_sum_parts(w, w.part0, a.heads, a.q_len, D, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh, st);
+        if (rc != YAMD_OK) return rc;
+    }
+    if (BIAS) {
+        hipLaunchKernelGGL(attention_bias_grad_kernel, dim3(ceil_div(a.n_off, 256), a.heads), dim3(256), 0, st, w, dbias);
+        YAMD_LAUNCH_CHECK();
+    }
+    return YAMD_OK;
+}
+
+}  // namespace
+}  // namespace yamd
+
+using namespace yamd;
+
+extern "C" size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *d, int biased)
+{
+    if (check_attention(d, nullptr, 0, nullptr) != YAMD_OK) return 0;
+    if (biased && (d->map_h <= 0 || d->map_w <= 0 || (long long)d->map_h * d->map_w != d->k_len)) return 0;
+    return plan_backward(d, biased != 0).workspace;
+}
+
+extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
+                                       const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,
+                                       const float *lse, const yamd_tokens *d_o, const yamd_tokens *dq, const yamd_tokens *dk,
+                                       const yamd_tokens *dv, float *dbias, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_attention(d, key_mask, mask_stride, bias);
+    if (rc == YAMD_OK) rc = check_tokens(d, q, d->q_len, d->heads, "q");
+    if (rc == YAMD_OK) rc = check_tokens(d, k, d->k_len, d->kv_heads, "k");
+    if (rc == YAMD_OK) rc = check_tokens(d, v, d->k_len, d->kv_heads, "v");
+    if (rc == YAMD_OK) rc = check_tokens(d, o, d->q_len, d->heads, "o");
+    if (rc == YAMD_OK) rc = check_tokens(d, d_o, d->q_len, d->heads, "do");
+    if (rc == YAMD_OK) rc = check_tokens(d, dq, d->q_len, d->heads, "dq");
+    if (rc == YAMD_OK) rc = check_tokens(d, dk, d->k_len, d->kv_heads, "dk");
+    if (rc == YAMD_OK) rc = check_tokens(d, dv, d->k_len, d->kv_heads, "dv");
+    if (rc != YAMD_OK) return rc;
+    YAMD_REQUIRE(lse, "attention backward: lse is null");
+    YAMD_REQUIRE((bias == nullptr) == (dbias == nullptr), "attention backward: bias and its gradient go together");
+    const BwdPlan p = plan_backward(d, bias != nullptr);
+    YAMD_REQUIRE(p.kv_total <= (1ll << 30) && p.q_total <= (1ll << 30), "attention backward: too many workgroups");
+    if (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15)) {
+        set_error("attention backward: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace ? workspace_bytes : (size_t)0, p.workspace);
+        return YAMD_ENOSPC;
+    }
+    AttnBwdArgs a = {};
+    a.q = view_of(q); a.k = view_of(k); a.v = view_of(v); a.o = view_of(o); a.go = view_of(d_o);
+    a.lse = lse;
+    a.delta = (float *)workspace;
+    a.part0 = (float *)((char *)workspace + p.delta);
+    a.part_bias = (float *)((char *)workspace + p.delta + p.parts);
+    a.ring = p.ring;
+    a.part_len = p.part_len;
+    a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
+    if (bias) {
+        a.map_w = d->map_w;
+        a.coord_last = map_coord(d->k_len - 1, d->map_w);
+        a.n_off = 2 * a.coord_last + 1;
+    }
+    a.batch = d->batch; a.q_len = d->q_len; a.k_len = d->k_len; a.d = d->head_dim;
+    a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads; a.scale = d->scale;
+    hipStream_t st = (hipStream_t)stream;
+    if (bias) {
+        switch (p.dpad) {
+        case 32: return launch_backward<32, true>(a, p, dq, dk, dv, dbias, st);
+        case 64: return launch_backward<64, true>(a, p, dq, dk, dv, dbias, st);
+        case 96: return launch_backward<96, true>(a, p, dq, dk, dv, dbias, st);
+        default: return launch_backward<128, true>(a, p, dq, dk, dv, dbias, st);
+        }
+    }
+    switch (p.dpad) {
+    case 32: return launch_backward<32, false>(a, p, dq, dk, dv, dbias, st);
+    case 64: return launch_backward<64, false>(a, p, dq, dk, dv, dbias, st);
+    case 96: return launch_backward<96, false>(a, p, dq, dk, dv, dbias, st);
+    default: return launch_backward<128, false>(a, p, dq, dk, dv, dbias, st);
+    }
+}

@@ -13,6 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libyolo_amd.so")
 
 ACT_NONE, ACT_SILU, ACT_LEAKY, ACT_MISH, ACT_RELU = 0, 1, 2, 3, 4
+DTYPE_F32, DTYPE_BF16 = 0, 1
 DECODE_V5, DECODE_V3, DECODE_POSE, DECODE_FACE = 0, 1, 2, 3
 
 # every symbol include/yolo_amd.h declares
@@ -23,6 +24,9 @@ EXPORTS = [
     "yamd_decode_anchor", "yamd_decode_anchor_levels", "yamd_decode_dfl", "yamd_decode_dfl_unit_conf", "yamd_decode_dfl_points", "yamd_nms_workspace_bytes", "yamd_nms_batched", "yamd_decode_nms_anchor", "yamd_nms_static_capacity_bytes", "yamd_nms_batched_static", "yamd_compact_rows", "yamd_letterbox_workspace_bytes", "yamd_letterbox_u8", "yamd_detect_match", "yamd_stem_packed_elems", "yamd_stem_pack_weights", "yamd_stem_conv", "yamd_stem_conv2_packed_elems", "yamd_stem_conv2_pack_weights", "yamd_stem_conv2",
     "yamd_bottleneck_packed_elems", "yamd_bottleneck_pack_weights", "yamd_bottleneck",
     "yamd_c3_packed_elems", "yamd_c3_pack_weights", "yamd_c3_fused",
+    "yamd_layer_norm", "yamd_layer_norm_backward_workspace_bytes", "yamd_layer_norm_backward",
+    "yamd_attention_workspace_bytes", "yamd_attention", "yamd_attention_backward_workspace_bytes", "yamd_attention_backward",
+    "yamd_relative_bias", "yamd_relative_bias_backward",
     "yamd_microbench_mfma_bf16", "yamd_microbench_copy", "yamd_microbench_clock_probe",
     "yamd_plan_create", "yamd_plan_run", "yamd_plan_size", "yamd_plan_destroy",
 ]
@@ -37,6 +41,17 @@ class ConvDesc(ctypes.Structure):
     _fields_ = [("ksize", c_int32), ("stride", c_int32), ("cin", c_int32), ("cout", c_int32), ("act", c_int32),
                 ("out_f32", c_int32), ("nrep", c_int32), ("ck", c_int32), ("mrep", c_int32), ("cout_pad", c_int32),
                 ("packed_w_elems", c_int64), ("nwaves", c_int32), ("residual_scale", ctypes.c_float), ("stages", c_int32)]
+
+
+class Tokens(ctypes.Structure):
+    """Mirror of ``yamd_tokens``."""
+    _fields_ = [("data", c_void_p), ("batch_stride", c_longlong), ("token_stride", c_longlong), ("head_stride", c_longlong)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """Mirror of ``yamd_attention_desc``."""
+    _fields_ = [("batch", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("q_len", c_int32),
+                ("k_len", c_int32), ("map_h", c_int32), ("map_w", c_int32), ("scale", c_float)]
 
 
 class PlanOp(ctypes.Structure):
@@ -130,6 +145,22 @@ def _load() -> ctypes.CDLL:
     lib.yamd_nms_static_capacity_bytes.argtypes = []
     lib.yamd_nms_batched_static.argtypes = [c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_double,
                                             c_void_p, c_void_p, c_int, c_void_p, c_void_p]
+    lib.yamd_layer_norm.argtypes = [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_float, c_void_p, c_longlong, c_void_p, c_void_p,
+                                    c_longlong, c_int, c_int, c_void_p]
+    lib.yamd_layer_norm_backward_workspace_bytes.restype = c_size_t
+    lib.yamd_layer_norm_backward_workspace_bytes.argtypes = [c_longlong, c_int]
+    lib.yamd_layer_norm_backward.argtypes = [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                             c_longlong, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_size_t, c_void_p]
+    T = P(Tokens)
+    lib.yamd_attention_workspace_bytes.restype = c_size_t
+    lib.yamd_attention_workspace_bytes.argtypes = [P(AttentionDesc), c_int]
+    lib.yamd_attention.argtypes = [P(AttentionDesc), T, T, T, c_void_p, c_longlong, c_void_p, T, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.yamd_attention_backward_workspace_bytes.restype = c_size_t
+    lib.yamd_attention_backward_workspace_bytes.argtypes = [P(AttentionDesc), c_int]
+    lib.yamd_attention_backward.argtypes = [P(AttentionDesc), T, T, T, c_void_p, c_longlong, c_void_p, T, c_void_p, T, T, T, T, c_void_p,
+                                            c_void_p, c_size_t, c_void_p]
+    lib.yamd_relative_bias.argtypes = [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]
+    lib.yamd_relative_bias_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p]
     lib.yamd_plan_create.argtypes = [P(PlanOp), c_int, c_int, c_int, c_int, P(c_void_p)]
     lib.yamd_plan_run.argtypes = [c_void_p, c_void_p, c_void_p, P(c_int)]
     lib.yamd_plan_size.argtypes = [c_void_p]
@@ -138,7 +169,8 @@ def _load() -> ctypes.CDLL:
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("yamd_plan_destroy","yamd_last_error", "yamd_nms_workspace_bytes", "yamd_letterbox_workspace_bytes", "yamd_stem_packed_elems", "yamd_stem_conv2_packed_elems", "yamd_bottleneck_packed_elems", "yamd_c3_packed_elems",
-                        "yamd_nms_static_capacity_bytes"):
+                        "yamd_nms_static_capacity_bytes", "yamd_layer_norm_backward_workspace_bytes", "yamd_attention_workspace_bytes",
+                        "yamd_attention_backward_workspace_bytes"):
             fn.restype = c_int
     return lib
 
