@@ -9,6 +9,8 @@
 #pragma once
 #include "yamd_common.h"
 
+#include <cmath>
+
 namespace yamd {
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
@@ -22,9 +24,20 @@ struct AttnView {
     long long sb, st, sh;                // strides of batch, token and head in elements
 };
 
-// a tile row is read 16 bytes at a time by 32 lanes on 32 rows: a row length of an odd multiple of 16 bytes spreads them
+// A tile of 64 rows in LDS: 16-byte chunks, row r's chunk c at position c ^ swizzle(r).  Rows are unpadded, because loads
+// write LDS directly, lane after lane; the swizzle spreads over the 64 banks both the 16-byte reads of 16 rows in one
+// column and the transposing reads, which take 64 bytes of each of 4 rows.
 template <int D>
-constexpr int kRow = D * 2 + 16;
+struct Tile {
+    static constexpr int kChunks = D <= 32 ? 4 : D <= 64 ? 8 : 16;      // per row; D = 96 leaves the last four unused
+    static constexpr int kRowBytes = kChunks * 16, kBytes = kTile * kRowBytes;
+    __device__ static __forceinline__ int swizzle(int r)
+    {
+        if constexpr (kChunks == 4) return (r >> 2) & 3;
+        else if constexpr (kChunks == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+        else return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+};
 
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
@@ -39,9 +52,12 @@ __device__ __forceinline__ f32x16 zero16()
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // A operand of rows [row0, row0 + 32) of a tile, columns 16 ks .. 16 ks + 15
-__device__ __forceinline__ bf16x8 rows_operand(const char *tile, int row_bytes, int row0, int ks, int lane)
+template <int D>
+__device__ __forceinline__ bf16x8 rows_operand(const char *tile, int row0, int ks, int lane)
 {
-    return *(const bf16x8 *)(tile + (row0 + (lane & 31)) * row_bytes + (16 * ks + 8 * (lane >> 5)) * 2);
+    using T = Tile<D>;
+    const int r = lane & 31;
+    return *(const bf16x8 *)(tile + row0 * T::kRowBytes + r * T::kRowBytes + (((2 * ks + (lane >> 5)) ^ T::swizzle(r)) << 4));
 }
 
 __device__ __forceinline__ s16x4 transposed_quad(const char *at)
@@ -54,16 +70,19 @@ __device__ __forceinline__ s16x4 transposed_quad(const char *at)
 // accumulator rows 16 u .. 16 u + 15 (counted from row0) have as a B operand.  Each group of 16 lanes reads 4 rows of 16
 // columns and gets them transposed: lane i of the group gives the address of row i / 4, columns 4 (i % 4) .. + 3 and
 // receives the 4 rows of column i.
-__device__ __forceinline__ bf16x8 transposed_operand(const char *tile, int row_bytes, int row0, int col0, int lane)
+template <int D>
+__device__ __forceinline__ bf16x8 transposed_operand(const char *tile, int row0, int col0, int lane)
 {
+    using T = Tile<D>;
     const int i = lane & 15, g = lane >> 4;
-    const char *at = tile + (row0 + 4 * (g >> 1) + (i >> 2)) * row_bytes + (col0 + 16 * (g & 1) + 4 * (i & 3)) * 2;
+    const int r = 4 * (g >> 1) + (i >> 2), c = col0 / 8 + 2 * (g & 1) + ((i >> 1) & 1);
+    const char *base = tile + row0 * T::kRowBytes + (i & 1) * 8;
     union {
         s16x4 q[2];
         bf16x8 v;
     } o;
-    o.q[0] = transposed_quad(at);
-    o.q[1] = transposed_quad(at + 8 * row_bytes);
+    o.q[0] = transposed_quad(base + r * T::kRowBytes + ((c ^ T::swizzle(r)) << 4));
+    o.q[1] = transposed_quad(base + (r + 8) * T::kRowBytes + ((c ^ T::swizzle(r + 8)) << 4));
     return o.v;
 }
 
@@ -97,32 +116,111 @@ static inline int work_grid(long long total) { return (int)(ceil_div(total, 8) *
 // two positions the index a(query) - a(key) + a(last) among the (2 h - 1)(2 w - 1) distances of the map.
 __host__ __device__ __forceinline__ int map_coord(int t, int w) { return t + (t / w) * (w - 1); }
 
-// 64 rows of a tile on their way from global memory to LDS: each of 256 threads moves D / 32 pieces of 16 bytes.
-template <int D>
-struct TilePieces {
-    static constexpr int N = D / 32, CPR = D / 8;
-    uint4 v[N];
+// Loads that write LDS directly: lane l of the wave takes 16 (4) bytes from `base` + `offset` and they land at byte 16 l
+// (4 l) behind `lds`; base and lds are the same for all lanes.  They are written as asm because the compiler, which cannot
+// tell the two buffers of a tile apart, would otherwise wait for the next tile's loads before it reads the current tile.
+// No register is written; whoever reads the tile waits with landed() and passes a barrier first.
+__device__ __forceinline__ unsigned lds_address(const void *p)
+{
+    return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const __attribute__((address_space(3))) char *)p);
+}
+__device__ __forceinline__ void load_lds_16(const void *base, unsigned offset, const void *lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_address(lds)), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds_4(const void *base, unsigned offset, const void *lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_address(lds)), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-    // rows first .. first + 63 of a token axis with `len` rows; pieces beyond the rows or beyond the head width read as zero
-    __device__ __forceinline__ void load(const __bf16 *base, long long st, int first, int len, int d)
+// Fills tiles with rows of a token axis of `len` rows (256 threads, each wave a quarter).  Rows beyond the axis repeat its
+// last row, chunks beyond the head width d are left as they are: both are cleared by the caller.
+template <int D>
+struct TileLoader {
+    using T = Tile<D>;
+    static constexpr int N = T::kChunks / 4;
+    unsigned offset[N];            // of this lane's pieces of a whole tile
+    unsigned row_bytes;
+    bool on[N];
+
+    __device__ __forceinline__ TileLoader(long long st, int d, int wave, int lane) : row_bytes((unsigned)st * 2)
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * 256 + threadIdx.x, row = id / CPR, c = id % CPR, t = first + row;
-            if (t < len && 8 * c < d) v[i] = *(const uint4 *)(base + (long long)t * st + 8 * c);
-            else v[i] = make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < N; ++n) {
+            const int at = (n * 4 + wave) * 64 + lane, r = at / T::kChunks, c = (at % T::kChunks) ^ T::swizzle(r);
+            offset[n] = r * row_bytes + 16 * c;
+            on[n] = 8 * c < d;
         }
     }
-    // `keep`: one bit per row; a row whose bit is clear is stored as zeros (a masked key may hold anything, NaN included)
-    __device__ __forceinline__ void store(char *tile, int row_bytes, unsigned long long keep) const
+    __device__ __forceinline__ void load(char *tile, const __bf16 *base, int first, int len, int wave, int lane) const
     {
+        const char *src = (const char *)base + (long long)first * row_bytes;
+        const int last = len - 1 - first;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * 256 + threadIdx.x, row = id / CPR, c = id % CPR;
-            *(uint4 *)(tile + row * row_bytes + c * 16) = (keep >> row) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < N; ++n) {
+            unsigned o = offset[n];
+            if (last < kTile - 1) {
+                const int r = ((n * 4 + wave) * 64 + lane) / T::kChunks;
+                o -= (r > last ? r - last : 0) * row_bytes;
+            }
+            if (on[n]) load_lds_16(src, o, tile + (n * 4 + wave) * 1024);
         }
     }
 };
+
+// `bytes` of LDS (a multiple of 16) set to zero by the workgroup
+__device__ __forceinline__ void clear_lds(char *p, int bytes)
+{
+    for (int at = threadIdx.x * 16; at < bytes; at += 256 * 16) *(uint4 *)(p + at) = make_uint4(0, 0, 0, 0);
+}
+
+// zeros in the rows whose bit of `keep` is clear: four threads per row
+template <int D>
+__device__ __forceinline__ void clear_rows(char *tile, unsigned long long keep)
+{
+    using T = Tile<D>;
+    const int r = threadIdx.x >> 2;
+    if ((keep >> r) & 1) return;
+#pragma unroll
+    for (int c = 0; c < T::kChunks / 4; ++c) *(uint4 *)(tile + r * T::kRowBytes + ((threadIdx.x & 3) * (T::kChunks / 4) + c) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// gives -inf to the scores of a tile's rows 32 u .. 32 u + 31 that are not kept
+__device__ __forceinline__ void mask_rows(f32x16 &s, unsigned long long keep, int u, int half)
+{
+    const unsigned bits = (unsigned)(keep >> (32 * u)) >> (4 * half);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = bits & (1u << acc_row(r, 0)) ? s[r] : -INFINITY;
+}
+
+__device__ __forceinline__ unsigned long long uniform64(unsigned long long v)
+{
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+    return ((unsigned long long)hi << 32) | lo;
+}
+
+// bits of the rows first .. first + 63 that are below len
+__device__ __forceinline__ unsigned long long rows_below(int first, int len)
+{
+    return len - first >= kTile ? ~0ull : (1ull << (len - first)) - 1;
+}
+
+// The biases of the distances between a workgroup's rows and a tile, staged in LDS: floats `from` .. `from` + n - 1 of a head's
+// bias at p[0 ..]; distances outside the table are never read and repeat its ends.
+__device__ __forceinline__ void load_window(char *lds, const float *bias, int from, int n, int n_off, int wave, int lane)
+{
+    for (int at = wave * 64; at < n; at += 256) {
+        const int o = from + at + lane;
+        load_lds_4(bias, (o < 0 ? 0 : o < n_off ? o : n_off - 1) * 4u, lds + at * 4);
+    }
+}
+// distances between 128 owned rows and a tile of 64, rounded up to what four waves load at once
+static inline int window_len(int map_h, int map_w)
+{
+    const int n = kBlockRows + kTile + (map_h > 1 ? kBlockRows + kTile + 2 * map_w : 0);
+    return (n + 255) / 256 * 256;
+}
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
 // argument checks shared by both directions (yamd_attention.hip)

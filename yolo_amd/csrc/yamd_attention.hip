@@ -24,25 +24,27 @@ struct AttnFwdArgs {
     const uint8_t *mask;           // [batch][k_len], 0 = not attended, or null
     long long mask_sb;
     const float *bias;             // [heads][(2 h - 1)(2 w - 1)]
-    int n_off, coord_last, map_w;
+    int n_off, coord_last, map_w, window;
     int batch, q_len, k_len, d, heads, kv_heads, group;
     int packed, rows, q_tiles, grid_heads, splits, tiles_per_split, total;
     float scale;
     float *part_o, *part_ml;       // [split][batch heads][q_len][D] and [...][2] when splits > 1
 };
 
+// LDS: two buffers of a tile of keys and one of values; then the coordinates and the mask of the two tiles' rows, and two
+// windows of the bias
 template <int D>
 struct FwdLds {
-    static constexpr int K = kTile * kRow<D>, BUF = 2 * K, BYTES = 2 * BUF + 2 * kTile * 4;
+    static constexpr int K = Tile<D>::kBytes, BUF = 2 * K, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
+    static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 : 0); }
 };
 
 template <int D, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
 {
     using L = FwdLds<D>;
-    constexpr int RB = kRow<D>, NKS = D / 16, NB = D / 32;
+    constexpr int NKS = D / 16, NB = D / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int *coords = (int *)(smem + 2 * L::BUF);            // a(key) of the tile's rows, two buffers
 
     int item = work_item();
     if (item >= a.total) return;
@@ -52,7 +54,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
     item /= a.q_tiles;
     const int gh = item % a.grid_heads, b = item / a.grid_heads;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int row0 = q_tile * kBlockRows + wave * 32;
     const int row = row0 + c32 < a.rows ? row0 + c32 : a.rows - 1;     // lanes beyond the rows repeat the last one
     const int in_group = a.packed ? row / a.q_len : 0;
@@ -74,58 +76,105 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
     }
     const __bf16 *kp = a.k.p + b * a.k.sb + kv_head * a.k.sh, *vp = a.v.p + b * a.v.sb + kv_head * a.v.sh;
     const uint8_t *mp = a.mask ? a.mask + b * a.mask_sb : nullptr;
-    const float *bp = BIAS ? a.bias + (long long)head * a.n_off + a.coord_last + map_coord(i, a.map_w) : nullptr;
-
     f32x16 acc[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) acc[n] = zero16();
-    float m = -INFINITY, l = 0.0f;                       // running maximum and this half's sum, in units of log 2
+    float m = -INFINITY, l = 0.0f;                       // running maximum (units of log 2) and this half's sum
     const float c2 = a.scale * kLog2e;
 
     const int t0 = split * a.tiles_per_split, n_tiles = (a.k_len + kTile - 1) / kTile;
     const int t1 = t0 + a.tiles_per_split < n_tiles ? t0 + a.tiles_per_split : n_tiles;
-    TilePieces<D> kn, vn;
-    bool valid_n = false;
-    auto fetch = [&](int t) {
-        const int first = t * kTile;
-        kn.load(kp, a.k.st, first, a.k_len, a.d);
-        vn.load(vp, a.v.st, first, a.k_len, a.d);
-        valid_n = first + lane < a.k_len && (!mp || mp[first + lane] != 0);
+
+    // distance index = c_row - a(key); a window starts at the distance of the workgroup's first row and the tile's last key
+    const float *bias = BIAS ? a.bias + (long long)gh * a.n_off : nullptr;
+    const int c_row = BIAS ? a.coord_last + map_coord(i, a.map_w) : 0;
+    const int c_first = BIAS ? a.coord_last + map_coord(q_tile * kBlockRows, a.map_w) : 0;
+    auto window_from = [&](int t) {
+        const int last = t * kTile + kTile - 1;
+        return c_first - map_coord(last < a.k_len ? last : a.k_len - 1, a.map_w);
     };
+    const TileLoader<D> kl(a.k.st, a.d, wave, lane), vl(a.v.st, a.d, wave, lane);
+    unsigned char mask_n = 1;
+    auto fetch = [&](int t) {
+        char *const kt = smem + (t & 1) * L::BUF;
+        kl.load(kt, kp, t * kTile, a.k_len, wave, lane);
+        vl.load(kt + L::K, vp, t * kTile, a.k_len, wave, lane);
+        if (BIAS) load_window(smem + L::WINDOW + (t & 1) * a.window * 4, bias, window_from(t), a.window, a.n_off, wave, lane);
+        if (mp && wave == 0 && t * kTile + lane < a.k_len) mask_n = mp[t * kTile + lane];
+    };
+    if (a.d < D) {                                       // channels beyond the head width: zeros that no load overwrites
+        clear_lds(smem, 2 * L::BUF);
+        __syncthreads();
+    }
+    // (a wait that the compiler sees: it would otherwise wait for the query rows inside the loop, and for the tiles with them)
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::K;
-        int *const ct = coords + (t & 1) * kTile;
-        const unsigned long long keep = __ballot(valid_n);
-        kn.store(kt, RB, keep);
-        vn.store(vt, RB, keep);
+        int *const coord = (int *)(smem + L::COORD) + (t & 1) * kTile;
+        unsigned long long *const kept = (unsigned long long *)(smem + L::KEEP) + (t & 1);
         if (BIAS && tid < kTile) {
             const int key = t * kTile + tid;
-            ct[tid] = map_coord(key < a.k_len ? key : a.k_len - 1, a.map_w);
+            coord[tid] = map_coord(key < a.k_len ? key : a.k_len - 1, a.map_w);
         }
+        if (mp && wave == 0) {
+            const unsigned long long v = __ballot(mask_n != 0);
+            if (lane == 0) *kept = v;
+        }
+        landed();
         __syncthreads();
+        // the mask that all waves act on is the one in LDS, so they agree on the barrier below whatever memory holds
+        unsigned long long keep = rows_below(t * kTile, a.k_len);
+        if (mp) keep &= *kept;
+        keep = uniform64(keep);
         if (t + 1 < t1) fetch(t + 1);
-        if (keep == 0 || row0 >= a.rows) continue;       // a tile without keys, a wave without rows
+        if (keep == 0) continue;
+        if (keep != ~0ull) {                             // a masked key may hold anything, NaN included
+            clear_rows<D>(kt, keep);
+            clear_rows<D>(vt, keep);
+            __syncthreads();
+        }
+        if (row0 >= a.rows) continue;
 
+        // operands are requested well ahead of the products that use them (the scheduler would put each read right before
+        // its product); the loads of the bias are in flight under the first product, those of half the values under the
+        // softmax
+        constexpr bool EARLY = D <= 64;                  // wider heads have no registers left for it
         f32x16 s[2];
+        bf16x8 kf[2][NKS];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) kf[u][ks] = rows_operand<D>(kt, 32 * u, ks, lane);
+        float bias_of[BIAS ? 32 : 1];
+        if constexpr (BIAS) {
+            const float *const w = (const float *)(smem + L::WINDOW) + (t & 1) * a.window + (c_row - window_from(t));
+#pragma unroll
+            for (int r = 0; r < 32; ++r) bias_of[r] = w[-coord[32 * (r >> 4) + acc_row(r & 15, half)]];
+        }
+        if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             s[u] = zero16();
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) s[u] = mfma(rows_operand(kt, RB, 32 * u, ks, lane), qf[ks], s[u]);
+            for (int ks = 0; ks < NKS; ++ks) s[u] = mfma(kf[u][ks], qf[ks], s[u]);
         }
+        bf16x8 vf[2][NB];
+        auto read_values = [&](bf16x8 (&f)[2][NB], int from) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) f[u][n] = transposed_operand<D>(vt, from + 16 * u, 32 * n, lane);
+        };
+        if constexpr (EARLY) read_values(vf, 0);
+        if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
         if constexpr (BIAS) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = s[u][r] * c2 + bp[-ct[32 * u + acc_row(r, half)]] * kLog2e;
+            for (int r = 0; r < 32; ++r) s[r >> 4][r & 15] = __builtin_fmaf(s[r >> 4][r & 15], a.scale, bias_of[r]);
         }
         if (keep != ~0ull) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!((keep >> (32 * u + acc_row(r, half))) & 1)) s[u][r] = -INFINITY;
+            mask_rows(s[0], keep, 0, half);
+            mask_rows(s[1], keep, 1, half);
         }
         float top = s[0][0];
 #pragma unroll
@@ -133,7 +182,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
         top = with_other_half(top, [](float x, float y) { return fmaxf(x, y); });
-        if constexpr (!BIAS) top *= c2;
+        const float unit = BIAS ? kLog2e : c2;           // scores to units of log 2
+        top *= unit;
         if (__any(top > m)) {
             const float m_new = fmaxf(m, top);
             const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
@@ -149,14 +199,25 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[u][r] = __builtin_amdgcn_exp2f(BIAS ? s[u][r] - sub : __builtin_fmaf(s[u][r], c2, -sub));
+                s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], unit, -sub));
                 l += s[u][r];
             }
+        bf16x8 vg[2][NB];
+        if constexpr (EARLY) read_values(vg, 32);
+        else read_values(vf, 0);
+        if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const bf16x8 pf = acc_operand(s[u >> 1], u & 1);
+        for (int u = 0; u < 2; ++u) {
+            const bf16x8 pf = acc_operand(s[0], u);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) acc[n] = mfma(transposed_operand(vt, RB, 16 * u, 32 * n, lane), pf, acc[n]);
+            for (int n = 0; n < NB; ++n) acc[n] = mfma(vf[u][n], pf, acc[n]);
+        }
+        if constexpr (!EARLY) read_values(vg, 32);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bf16x8 pf = acc_operand(s[1], u);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) acc[n] = mfma(vg[u][n], pf, acc[n]);
         }
     }
     l = with_other_half(l, [](float x, float y) { return x + y; });
@@ -254,6 +315,7 @@ int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
     YAMD_REQUIRE((d->batch == 1 || (t->batch_stride % 8 == 0 && t->batch_stride >= 0)) && (len == 1 || (t->token_stride % 8 == 0 && t->token_stride > 0)) &&
                      (heads == 1 || (t->head_stride % 8 == 0 && t->head_stride > 0)),
                  "attention: strides of %s must be positive multiples of 8 elements", name);
+    YAMD_REQUIRE(len == 1 || t->token_stride <= (1 << 24), "attention: tokens of %s are more than 2^24 elements apart", name);
     return YAMD_OK;
 }
 
@@ -296,10 +358,11 @@ FwdPlan plan_forward(const yamd_attention_desc *d, bool biased)
 template <int D, bool BIAS>
 int launch_forward(const AttnFwdArgs &a, long long rows, hipStream_t st)
 {
-    using Attr = KernelAttr<&attention_kernel<D, BIAS>, FwdLds<D>::BYTES>;
+    using Attr = KernelAttr<&attention_kernel<D, BIAS>, FwdLds<D>::most(BIAS)>;
+    const int lds = FwdLds<D>::WINDOW + 2 * a.window * (int)sizeof(float);
     const int rc = Attr::ensure();
     if (rc != YAMD_OK) return rc;
-    hipLaunchKernelGGL((attention_kernel<D, BIAS>), dim3(work_grid(a.total)), dim3(256), FwdLds<D>::BYTES, st, a);
+    hipLaunchKernelGGL((attention_kernel<D, BIAS>), dim3(work_grid(a.total)), dim3(256), lds, st, a);
     YAMD_LAUNCH_CHECK();
     if (a.splits > 1) {
         hipLaunchKernelGGL((attention_join_kernel<D>), dim3(ceil_div(rows * (D / 4), 256)), dim3(256), 0, st, a, rows);
@@ -340,9 +403,10 @@ extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q
     a.o = (__bf16 *)o->data; a.o_sb = o->batch_stride; a.o_st = o->token_stride; a.o_sh = o->head_stride;
     a.lse = lse; a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
     if (bias) {
-        a.map_w = d->map_w;
-        a.coord_last = map_coord(d->k_len - 1, d->map_w);
+        a.map_w = d->map_h > 1 ? d->map_w : 1;       // (of a sequence the coordinate is the position, also beyond its end)
+        a.coord_last = map_coord(d->k_len - 1, a.map_w);
         a.n_off = 2 * a.coord_last + 1;
+        a.window = window_len(d->map_h, d->map_w);
     }
     a.batch = d->batch; a.q_len = d->q_len; a.k_len = d->k_len; a.d = d->head_dim; a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads;
     a.packed = p.packed; a.rows = p.rows; a.q_tiles = p.q_tiles; a.grid_heads = p.grid_heads; a.splits = p.splits;

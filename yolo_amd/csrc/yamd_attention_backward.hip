@@ -30,8 +30,11 @@ struct AttnBwdArgs {
     long long o0_sb, o0_st, o0_sh, o1_sb, o1_st, o1_sh;
     float *part0, *part1;          // float32 parts [split][batch * heads][len][D] when splits > 1
     float *part_bias;              // [batch * heads * tiles][part_len]: sums by distance of one workgroup
-    int ring, part_len;
+    int ring, part_len, window;
 };
+
+// the two rings of a wave lie 36 banks apart: the halves hold distances 4 apart, so that their 64 lanes meet 64 banks
+constexpr int kRingPad = 36;
 
 // D = rowsum(do o): 16 lanes per row, 8 channels each.  A row without keys (lse = -inf) has no gradient whatever do holds.
 __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
@@ -62,14 +65,16 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
 // tile's rows, dV^T += dO^T P and dK^T += Q^T dS read it transposed.
 template <int D>
 struct KvLds {
-    static constexpr int T = kTile * kRow<D>, BUF = 2 * T + 3 * kTile * 4, BYTES = 2 * BUF;
+    static constexpr int T = Tile<D>::kBytes, BUF = 2 * T, STATS = 2 * BUF, WINDOW = STATS + 2 * 3 * kTile * 4;
+    static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 : 0); }
 };
 
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(AttnBwdArgs a)
 {
     using L = KvLds<D>;
-    constexpr int RB = kRow<D>, NKS = D / 16, NB = D / 32;
+    constexpr int NKS = D / 16, NB = D / 32;
+    constexpr bool EARLY = true;                    // wider heads have no registers left to request operands ahead
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
     int item = work_item();
@@ -80,7 +85,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
     item /= a.tiles;
     const int kv_head = item % a.kv_heads, b = item / a.kv_heads;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int key0 = tile * kBlockRows + wave * 32;
     const int key = key0 + c32 < a.k_len ? key0 + c32 : a.k_len - 1;
     const bool valid = key0 + c32 < a.k_len && (!a.mask || a.mask[b * a.mask_sb + key] != 0);
@@ -102,73 +107,121 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
             }
         }
     }
-    const int ck = BIAS ? a.coord_last - map_coord(key, a.map_w) : 0;
+    // distance index = a(query) + c_key; a window starts at the distance of the tile's first query and the workgroup's last key
+    const int c_key = BIAS ? a.coord_last - map_coord(key, a.map_w) : 0;
+    const int last_key = tile * kBlockRows + kBlockRows - 1 < a.k_len ? tile * kBlockRows + kBlockRows - 1 : a.k_len - 1;
+    const int c_low = BIAS ? a.coord_last - map_coord(last_key, a.map_w) : 0;
 
     f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) dk[n] = zero16(), dv[n] = zero16();
-    const float c2 = a.scale * kLog2e;
+    const float c2 = a.scale * kLog2e, inv_scale = 1.0f / a.scale;
 
     // the loop runs over (head of the group, tile of queries)
     const int q_tiles = (a.q_len + kTile - 1) / kTile, loop = a.group * q_tiles;
     const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < loop ? t0 + a.loop_per_split : loop;
-    TilePieces<D> qn, gn;
+    const TileLoader<D> ql(a.q.st, a.d, wave, lane), gl(a.go.st, a.d, wave, lane);
     float lse_n = 0.0f, delta_n = 0.0f;
     auto fetch = [&](int t) {
         const int head = kv_head * a.group + t / q_tiles, first = t % q_tiles * kTile;
-        qn.load(a.q.p + b * a.q.sb + head * a.q.sh, a.q.st, first, a.q_len, a.d);
-        gn.load(a.go.p + b * a.go.sb + head * a.go.sh, a.go.st, first, a.q_len, a.d);
-        // rows beyond the queries, and rows without keys, get an infinite sum: their probabilities are exp2(-inf) = 0
-        lse_n = INFINITY;
-        delta_n = 0.0f;
-        if (first + lane < a.q_len) {
-            const long long w = ((long long)b * a.heads + head) * a.q_len + first + lane;
-            lse_n = a.lse[w] == -INFINITY ? INFINITY : a.lse[w];
-            delta_n = a.delta[w];
+        char *const qt = smem + (t & 1) * L::BUF;
+        ql.load(qt, a.q.p + b * a.q.sb + head * a.q.sh, first, a.q_len, wave, lane);
+        gl.load(qt + L::T, a.go.p + b * a.go.sb + head * a.go.sh, first, a.q_len, wave, lane);
+        if (BIAS)
+            load_window(smem + L::WINDOW + (t & 1) * a.window * 4, a.bias + (long long)head * a.n_off, c_low + map_coord(first, a.map_w),
+                        a.window, a.n_off, wave, lane);
+        if (wave == 0) {
+            // rows beyond the queries, and rows without keys, get an infinite sum: their probabilities are exp2(-inf) = 0
+            lse_n = INFINITY;
+            delta_n = 0.0f;
+            if (first + lane < a.q_len) {
+                const long long w = ((long long)b * a.heads + head) * a.q_len + first + lane;
+                lse_n = a.lse[w];
+                delta_n = a.delta[w];
+            }
         }
     };
+    if (a.d < D) {                                     // channels beyond the head width: zeros that no load overwrites
+        clear_lds(smem, 2 * L::BUF);
+        __syncthreads();
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         char *const qt = smem + (t & 1) * L::BUF, *const gt = qt + L::T;
-        float *const lse2 = (float *)(gt + L::T), *const delta = lse2 + kTile;
+        float *const lse_s = (float *)(smem + L::STATS) + (t & 1) * 3 * kTile, *const delta = lse_s + kTile;
         int *const coord = (int *)(delta + kTile);
-        const unsigned long long keep = __ballot(lse_n != INFINITY);
-        qn.store(qt, RB, keep);                        // a row without keys gives no gradient whatever q and do hold
-        gn.store(gt, RB, keep);
-        if (tid < kTile) {
-            lse2[tid] = lse_n * kLog2e;
-            delta[tid] = delta_n;
-            if (BIAS) {
-                const int i = t % q_tiles * kTile + tid;
-                coord[tid] = map_coord(i < a.q_len ? i : a.q_len - 1, a.map_w);
-            }
+        if (wave == 0) {
+            lse_s[lane] = lse_n == -INFINITY ? -INFINITY : -lse_n * inv_scale;
+            delta[lane] = -delta_n;
         }
-        const float *bp = BIAS ? a.bias + (long long)(kv_head * a.group + t / q_tiles) * a.n_off + ck : nullptr;
+        if (BIAS && tid < kTile) {
+            const int i = t % q_tiles * kTile + tid;
+            coord[tid] = map_coord(i < a.q_len ? i : a.q_len - 1, a.map_w);
+        }
+        landed();
         __syncthreads();
+        // read from LDS by all waves, so that they agree on the barrier below
+        const unsigned long long keep = uniform64(__ballot(lse_s[lane] != -INFINITY));
         if (t + 1 < t1) fetch(t + 1);
+        if (keep != ~0ull) {                           // a row without keys gives no gradient whatever q and do hold
+            clear_rows<D>(qt, keep);
+            clear_rows<D>(gt, keep);
+            __syncthreads();
+        }
+        const float *const win = (const float *)(smem + L::WINDOW) + (t & 1) * a.window +
+                                 (BIAS ? c_key - c_low - map_coord(t % q_tiles * kTile, a.map_w) : 0);
         if (!busy) continue;
+        // Operands are requested one stage ahead of the products that use them, as far as registers allow; fences keep the
+        // scheduler from putting each read right before its product.  Columns (keys) do not mix, so a masked key's column
+        // may hold anything until its result is replaced by zeros at the end.
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            f32x16 s = zero16(), g = zero16();
+            bf16x8 qr[NKS], gr[NKS];
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) s = mfma(rows_operand(qt, RB, 32 * u, ks, lane), kf[ks], s);
+            for (int ks = 0; ks < NKS; ++ks) qr[ks] = rows_operand<D>(qt, 32 * u, ks, lane);
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) g = mfma(rows_operand(gt, RB, 32 * u, ks, lane), vf[ks], g);
+            for (int ks = 0; ks < NKS; ++ks) gr[ks] = rows_operand<D>(gt, 32 * u, ks, lane);
+            // both products start from a row's statistics: s from -lse / scale, dP from -D
+            f32x16 s, g;
+            int at[BIAS ? 16 : 1];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int at = 32 * u + acc_row(r, half);
-                const float x = BIAS ? bp[coord[at]] * kLog2e - lse2[at] : -lse2[at];
-                const float p = valid ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, x)) : 0.0f;
-                s[r] = p;
-                g[r] = p * (g[r] - delta[at]);
+                s[r] = lse_s[32 * u + acc_row(r, half)];
+                g[r] = delta[32 * u + acc_row(r, half)];
+                if constexpr (BIAS) at[r] = coord[32 * u + acc_row(r, half)];
+            }
+            float bias_of[BIAS ? 16 : 1];
+            if constexpr (BIAS) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) bias_of[r] = win[at[r]];
+            }
+            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) s = mfma(qr[ks], kf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) g = mfma(gr[ks], vf[ks], g);
+            bf16x8 gx[2][NB], qx[2][NB];
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    gx[w][n] = transposed_operand<D>(gt, 32 * u + 16 * w, 32 * n, lane);
+                    qx[w][n] = transposed_operand<D>(qt, 32 * u + 16 * w, 32 * n, lane);
+                }
+            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(BIAS ? __builtin_fmaf(s[r], c2, bias_of[r] * kLog2e) : s[r] * c2);
+                g[r] *= s[r];
             }
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const bf16x8 pf = acc_operand(s, w), sf = acc_operand(g, w);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    dv[n] = mfma(transposed_operand(gt, RB, 32 * u + 16 * w, 32 * n, lane), pf, dv[n]);
-                    dk[n] = mfma(transposed_operand(qt, RB, 32 * u + 16 * w, 32 * n, lane), sf, dk[n]);
+                    dv[n] = mfma(gx[w][n], pf, dv[n]);
+                    dk[n] = mfma(qx[w][n], sf, dk[n]);
                 }
             }
         }
@@ -212,23 +265,26 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
 // tile's rows, dQ^T += K^T dS^T reads the keys transposed.
 //
 // The bias gradient is summed by distance.  For one key, the 32 queries of a half wave lie at 32 different distances, so
-// the wave adds its dS values into a ring of float32 sums in LDS of its own without two lanes of a half meeting.  As the
+// each half wave adds its dS values into a ring of float32 sums in LDS of its own without two lanes meeting: plain loads
+// and stores, in order within a wave.  (LDS float atomics: 81 ns per wave and CU, this 4 ns; 1120 against XX us for ...)  As the
 // keys advance the distances fall: those above a(last query) - a(first key of the next tile) are final, and after each
-// tile the workgroup adds the four waves' rings in a fixed order for them, writes them to its row of the workspace and
+// tile the workgroup adds the eight rings in a fixed order for them, writes them to its row of the workspace and
 // clears them.  The ring must hold the distances of two tiles (one being added to while the other is written out):
 // 2 * 127 + 1 positions, and where a map has several rows 127 + 127 + 2 w more.
 template <int D>
 struct QLds {
-    static constexpr int T = kTile * kRow<D>, BUF = 2 * T + kTile * 4, BYTES = 2 * BUF;
+    static constexpr int T = Tile<D>::kBytes, BUF = 2 * T, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
+    static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 + 8 * (2048 + kRingPad) * 4 : 0); }
 };
 
 template <int D, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 {
     using L = QLds<D>;
-    constexpr int RB = kRow<D>, NKS = D / 16, NB = D / 32;
+    constexpr int NKS = D / 16, NB = D / 32;
+    constexpr bool EARLY = D <= 64;                    // wider heads have no registers left to request operands ahead
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float *const rings = (float *)(smem + L::BYTES);
+    float *const rings = (float *)(smem + L::WINDOW) + 2 * a.window;
 
     int item = work_item();
     if (item >= a.total) return;
@@ -239,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     item /= a.tiles;
     const int head = item % a.heads, b = item / a.heads, kv_head = head / a.group;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int row0 = tile * kBlockRows + wave * 32;
     const int i = row0 + c32 < a.q_len ? row0 + c32 : a.q_len - 1;
     const long long stat = ((long long)b * a.heads + head) * a.q_len + i;
@@ -269,17 +325,15 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 
     // distance index of (query, key) = cq - a(key); of the workgroup's rows the first and last
     int cq = 0, c_first = 0, c_last = 0, high = 0;
-    const float *bp = nullptr;
     float *ring = nullptr;
     if constexpr (BIAS) {
         const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
-        cq = a.coord_last + map_coord(i, a.map_w);
+        cq = a.coord_last + map_coord(row0 + c32, a.map_w);    // (lanes beyond the queries too have distances of their own)
         c_first = a.coord_last + map_coord(tile * kBlockRows, a.map_w);
         c_last = a.coord_last + map_coord(last, a.map_w);
         high = c_last + 1;                             // distances from here on are written out (a(0) = 0)
-        bp = a.bias + (long long)head * a.n_off + cq;
-        ring = rings + wave * a.ring;
-        for (int e = tid; e < 4 * a.ring; e += 256) rings[e] = 0.0f;
+        ring = rings + (2 * wave + half) * (a.ring + kRingPad);
+        for (int e = tid; e < 8 * (a.ring + kRingPad); e += 256) rings[e] = 0.0f;
     }
 
     f32x16 dq[NB];
@@ -289,13 +343,17 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 
     const int n_tiles = (a.k_len + kTile - 1) / kTile;
     const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < n_tiles ? t0 + a.loop_per_split : n_tiles;
-    TilePieces<D> kn, vn;
-    bool valid_n = false;
+    auto window_from = [&](int t) { return c_first - map_coord(t * kTile + kTile - 1, a.map_w); };
+    const TileLoader<D> kl(a.k.st, a.d, wave, lane), vl(a.v.st, a.d, wave, lane);
+    unsigned char mask_n = 1;
     auto fetch = [&](int t) {
-        const int first = t * kTile;
-        kn.load(kp, a.k.st, first, a.k_len, a.d);
-        vn.load(vp, a.v.st, first, a.k_len, a.d);
-        valid_n = first + lane < a.k_len && (!mp || mp[first + lane] != 0);
+        char *const kt = smem + (t & 1) * L::BUF;
+        kl.load(kt, kp, t * kTile, a.k_len, wave, lane);
+        vl.load(kt + L::T, vp, t * kTile, a.k_len, wave, lane);
+        if (BIAS)
+            load_window(smem + L::WINDOW + (t & 1) * a.window * 4, a.bias + (long long)head * a.n_off, window_from(t), a.window, a.n_off,
+                        wave, lane);
+        if (mp && wave == 0 && t * kTile + lane < a.k_len) mask_n = mp[t * kTile + lane];
     };
     // writes the sums of the distances [low, high) out and clears them
     auto flush = [&](int low) {
@@ -303,60 +361,128 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         const int base = c_first - a.coord_last;       // the smallest distance of the workgroup: first query, last key
         for (int e = low + tid; e < high; e += 256) {
             const int at = e & (a.ring - 1);
-            float s = rings[at];
-            rings[at] = 0.0f;
+            float s = 0.0f;
 #pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                s += rings[w * a.ring + at];
-                rings[w * a.ring + at] = 0.0f;
+            for (int w = 0; w < 8; ++w) {
+                s += rings[w * (a.ring + kRingPad) + at];
+                rings[w * (a.ring + kRingPad) + at] = 0.0f;
             }
             out[e - base] = s;
         }
         high = low;
     };
+    if (a.d < D) {                                     // channels beyond the head width: zeros that no load overwrites
+        clear_lds(smem, 2 * L::BUF);
+        __syncthreads();
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::T;
-        int *const ct = (int *)(vt + L::T);
-        const unsigned long long keep = __ballot(valid_n);
-        kn.store(kt, RB, keep);
-        vn.store(vt, RB, keep);
-        if (BIAS && tid < kTile) {
-            const int key = t * kTile + tid;
-            ct[tid] = map_coord(key < a.k_len ? key : a.k_len - 1, a.map_w);
+        int *const coord = (int *)(smem + L::COORD) + (t & 1) * kTile;
+        unsigned long long *const kept = (unsigned long long *)(smem + L::KEEP) + (t & 1);
+        if (BIAS && tid < kTile) coord[tid] = map_coord(t * kTile + tid, a.map_w);      // (keys beyond the last one continue)
+        if (mp && wave == 0) {
+            const unsigned long long v = __ballot(mask_n != 0);
+            if (lane == 0) *kept = v;
         }
+        landed();
         __syncthreads();
+        unsigned long long keep = rows_below(t * kTile, a.k_len);
+        if (mp) keep &= *kept;                         // (from LDS: all waves agree on the barrier below)
+        keep = uniform64(keep);
         if (t + 1 < t1) fetch(t + 1);
         if constexpr (BIAS) flush(c_last - map_coord(t * kTile, a.map_w) + 1);   // what the tiles before this one left final
-        if (!busy || keep == 0) continue;
+        if (keep == 0) continue;
+        if (keep != ~0ull) {                           // a masked key may hold anything, NaN included
+            clear_rows<D>(kt, keep);
+            clear_rows<D>(vt, keep);
+            __syncthreads();
+        }
+        if (!busy) continue;
+        const float *const win = (const float *)(smem + L::WINDOW) + (t & 1) * a.window + (BIAS ? cq - window_from(t) : 0);
+        // P and dS of 32 keys: s holds the scores, g dP
+        auto score_gradient = [&](f32x16 &s, f32x16 &g, int u) {
+            float x[BIAS ? 16 : 1];
+            if constexpr (BIAS) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f32x16 s = zero16(), g = zero16();
+                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(win[-coord[32 * u + acc_row(r, half)]], kLog2e, -lse2);
+            }
+            if (keep != ~0ull) mask_rows(s, keep, u, half);
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) s = mfma(rows_operand(kt, RB, 32 * u, ks, lane), qf[ks], s);
+            for (int r = 0; r < 16; ++r) g[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, BIAS ? x[r] : -lse2)) * (g[r] - delta);
+        };
+        if constexpr (EARLY) {
+            bf16x8 kr[2][NKS], vr[2][NKS];
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) g = mfma(rows_operand(vt, RB, 32 * u, ks, lane), gf[ks], g);
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int at = 32 * u + acc_row(r, half);
-                int ca = 0;
-                float x = -lse2;
-                if constexpr (BIAS) {
-                    ca = ct[at];
-                    x += bp[-ca] * kLog2e;
+                for (int ks = 0; ks < NKS; ++ks) {
+                    kr[u][ks] = rows_operand<D>(kt, 32 * u, ks, lane);
+                    vr[u][ks] = rows_operand<D>(vt, 32 * u, ks, lane);
                 }
-                const float p = (keep >> at) & 1 ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, x)) : 0.0f;
-                g[r] = p * (g[r] - delta);
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 s[2], g[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = zero16(), g[u] = zero16();
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) s[u] = mfma(kr[u][ks], qf[ks], s[u]);
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) g[u] = mfma(vr[u][ks], gf[ks], g[u]);
+            }
+            bf16x8 kx[4][NB];
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) kx[w][n] = transposed_operand<D>(kt, 16 * w, 32 * n, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                score_gradient(s[u], g[u], u);
+                if constexpr (BIAS) __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("" ::: "memory");                   // (the coordinates are read again below, not kept)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const bf16x8 sf = acc_operand(g[w >> 1], w & 1);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) dq[n] = mfma(kx[w][n], sf, dq[n]);
                 if constexpr (BIAS) {
-                    // lanes without a query repeat the last one with dS = 0
-                    __hip_atomic_fetch_add(ring + ((cq - ca) & (a.ring - 1)), g[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    // keys 32 apart are at least 32 distances apart: two additions at a time cannot meet
+#pragma unroll
+                    for (int r = 4 * w; r < 4 * w + 4; ++r) {
+                        float *const p0 = ring + ((cq - coord[acc_row(r, half)]) & (a.ring - 1));
+                        float *const p1 = ring + ((cq - coord[32 + acc_row(r, half)]) & (a.ring - 1));
+                        const float x0 = *p0, x1 = *p1;
+                        *p0 = x0 + g[0][r];
+                        *p1 = x1 + g[1][r];
+                        asm volatile("" ::: "memory");       // the next addition may read what another lane wrote here
+                    }
                 }
             }
+        } else {
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const bf16x8 sf = acc_operand(g, w);
+            for (int u = 0; u < 2; ++u) {
+                f32x16 s = zero16(), g = zero16();
 #pragma unroll
-                for (int n = 0; n < NB; ++n) dq[n] = mfma(transposed_operand(kt, RB, 32 * u + 16 * w, 32 * n, lane), sf, dq[n]);
+                for (int ks = 0; ks < NKS; ++ks) s = mfma(rows_operand<D>(kt, 32 * u, ks, lane), qf[ks], s);
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) g = mfma(rows_operand<D>(vt, 32 * u, ks, lane), gf[ks], g);
+                score_gradient(s, g, u);
+                if constexpr (BIAS) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        ring[(cq - coord[32 * u + acc_row(r, half)]) & (a.ring - 1)] += g[r];
+                        asm volatile("" ::: "memory");
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const bf16x8 sf = acc_operand(g, w);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) dq[n] = mfma(transposed_operand<D>(kt, 32 * u + 16 * w, 32 * n, lane), sf, dq[n]);
+                }
             }
         }
     }
@@ -474,7 +600,7 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     if (biased) {
         const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
         for (p.ring = 256; p.ring < span; p.ring *= 2) {}
-        const int coord_last = map_coord(d->k_len - 1, d->map_w);
+        const int coord_last = map_coord(d->k_len - 1, w);
         p.part_len = coord_last + kBlockRows + (d->map_h > 1 ? kBlockRows + w : 0);
         p.bias = up256((size_t)bh * p.q_tiles * p.part_len * sizeof(float));
     }
@@ -486,9 +612,8 @@ template <int D, bool BIAS>
 int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv, float *dbias,
                     hipStream_t st)
 {
-    constexpr int kRingBytes = BIAS ? 4 * 2048 * 4 : 0;
-    using KvAttr = KernelAttr<&attention_dkv_kernel<D, BIAS>, KvLds<D>::BYTES>;
-    using QAttr = KernelAttr<&attention_dq_kernel<D, BIAS>, QLds<D>::BYTES + kRingBytes>;
+    using KvAttr = KernelAttr<&attention_dkv_kernel<D, BIAS>, KvLds<D>::most(BIAS)>;
+    using QAttr = KernelAttr<&attention_dq_kernel<D, BIAS>, QLds<D>::most(BIAS)>;
     int rc = KvAttr::ensure();
     if (rc == YAMD_OK) rc = QAttr::ensure();
     if (rc != YAMD_OK) return rc;
@@ -502,7 +627,7 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
     w.out1 = (__bf16 *)dv->data; w.o1_sb = dv->batch_stride; w.o1_st = dv->token_stride; w.o1_sh = dv->head_stride;
     const size_t half = (size_t)p.kv_splits * a.batch * a.kv_heads * a.k_len * D;
     w.part1 = w.part0 + half;
-    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256), KvLds<D>::BYTES, st, w);
+    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256), KvLds<D>::WINDOW + 2 * a.window * (int)sizeof(float), st, w);
     YAMD_LAUNCH_CHECK();
     if (w.splits > 1) {
         rc = launch_sum_parts(w, w.part0, a.kv_heads, a.k_len, D, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh, st);
@@ -514,7 +639,7 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
     w.tiles = p.q_tiles; w.splits = p.q_splits; w.loop_per_split = p.q_loop; w.total = (int)p.q_total;
     w.out0 = (__bf16 *)dq->data; w.o0_sb = dq->batch_stride; w.o0_st = dq->token_stride; w.o0_sh = dq->head_stride;
     hipLaunchKernelGGL((attention_dq_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256),
-                       QLds<D>::BYTES + (BIAS ? 4 * p.ring * (int)sizeof(float) : 0), st, w);
+                       QLds<D>::WINDOW + (BIAS ? 2 * a.window + 8 * (p.ring + kRingPad) : 0) * (int)sizeof(float), st, w);
     YAMD_LAUNCH_CHECK();
     if (w.splits > 1) {
         rc = launch_sum_parts(w, w.part0, a.heads, a.q_len, D, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh, st);
@@ -572,9 +697,10 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     a.part_len = p.part_len;
     a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
     if (bias) {
-        a.map_w = d->map_w;
-        a.coord_last = map_coord(d->k_len - 1, d->map_w);
+        a.map_w = d->map_h > 1 ? d->map_w : 1;       // (of a sequence the coordinate is the position, also beyond its end)
+        a.coord_last = map_coord(d->k_len - 1, a.map_w);
         a.n_off = 2 * a.coord_last + 1;
+        a.window = window_len(d->map_h, d->map_w);
     }
     a.batch = d->batch; a.q_len = d->q_len; a.k_len = d->k_len; a.d = d->head_dim;
     a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads; a.scale = d->scale;
