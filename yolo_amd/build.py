@@ -1,4 +1,5 @@
-"""Builds yolo_amd/libyolo_amd.so from yolo_amd/csrc/*.hip with hipcc for gfx950.
+"""Builds yolo_amd/libyolo_amd.so from yolo_amd/csrc/*.hip with hipcc for gfx950, and yolo_amd/_torch_ops.so, the torch
+binding of the token operators, from csrc/yamd_torch.cpp with the host compiler.
 
 The library is built in-tree so the same file is what tests, bench.py and smoke() load; there is
 no JIT and no fallback: if the .so is missing, ``yolo_amd.lib`` raises.
@@ -46,6 +47,10 @@ HEADERS = [os.path.join(CSRC, "yamd_common.h"), os.path.join(CSRC, "yamd_conv_ke
            os.path.join(HERE, "..", "include", "yolo_amd.h")]
 
 
+BINDING_SRC = os.path.join(CSRC, "yamd_torch.cpp")
+BINDING = os.path.join(HERE, "_torch_ops.so")
+
+
 def _hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", "hipcc"):
         if cand and (os.path.isabs(cand) and os.path.exists(cand) or not os.path.isabs(cand)):
@@ -85,6 +90,29 @@ def build_library(force: bool = False, verbose: bool = True) -> str:
     return LIB
 
 
+def build_binding(force: bool = False, verbose: bool = True) -> str:
+    """Host code over the C ABI and torch's C++ API; needs libyolo_amd.so to link against."""
+    header = os.path.join(HERE, "..", "include", "yolo_amd.h")
+    if not force and not _stale(BINDING, [BINDING_SRC, header]):
+        return BINDING
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for inc in include_paths() + [os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]:
+        cmd += ["-isystem", inc]
+    cmd += [BINDING_SRC, "-o", BINDING, "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+            "-L" + HERE, "-l:libyolo_amd.so", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print("[yolo_amd.build]", " ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return BINDING
+
+
 if __name__ == "__main__":
     build_library(force="--force" in sys.argv)
+    build_binding(force="--force" in sys.argv)
     print(LIB)
