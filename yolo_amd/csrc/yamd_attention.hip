@@ -252,38 +252,59 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         a.lse[((long long)b * a.heads + head) * a.q_len + i] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
-// joins the parts of a split key axis: one thread per (row, 4 channels)
+// Joins the parts of a split key axis: one wave per row.  A lane owns 4 channels, and the 64 / (D / 4) groups of lanes take
+// the parts in turns, four at a time so that their loads overlap; the groups are joined by exchanges in a fixed order.
 template <int D>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long long rows)
 {
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long at = id / (D / 4);
-    const int c = (int)(id % (D / 4)) * 4;
+    constexpr int CH = D == 96 ? 32 : D / 4, G = 64 / CH;      // (of 32 lanes 24 work for D = 96)
+    const int lane = threadIdx.x & 63, g = lane / CH, c = 4 * (lane % CH);
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= rows) return;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + at)]);
-    const float sub = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
+    float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = *(const float2 *)(a.part_ml + 2 * (s * rows + at));
-        const float f = __builtin_amdgcn_exp2f(ml.x - sub);
-        l += ml.y * f;
-        const f32x4 p = *(const f32x4 *)(a.part_o + (s * rows + at) * D + c);
-        o += p * f;
+    auto merge = [&](float pm, float pl, f32x4 po) {
+        const float m_new = fmaxf(m, pm), sub = m_new == -INFINITY ? 0.0f : m_new;
+        const float f = __builtin_amdgcn_exp2f(m - sub), pf = __builtin_amdgcn_exp2f(pm - sub);
+        m = m_new;
+        l = l * f + pl * pf;
+        o = o * f + po * pf;
+    };
+    for (int s0 = g; s0 < a.splits; s0 += 4 * G) {
+        float2 ml[4];
+        f32x4 po[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = s0 + k * G;
+            ml[k] = make_float2(-INFINITY, 0.0f);
+            po[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (s < a.splits) {
+                ml[k] = *(const float2 *)(a.part_ml + 2 * (s * rows + at));
+                if (c < D) po[k] = *(const f32x4 *)(a.part_o + (s * rows + at) * D + c);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) merge(ml[k].x, ml[k].y, po[k]);
+    }
+#pragma unroll
+    for (int d = CH; d < 64; d <<= 1) {
+        const float pm = __shfl_xor(m, d), pl = __shfl_xor(l, d);
+        f32x4 po;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) po[e] = __shfl_xor(o[e], d);
+        merge(pm, pl, po);
     }
     const int i = (int)(at % a.q_len);
     const long long bh = at / a.q_len;
     const int head = (int)(bh % a.heads);
-    const long long b = bh / a.heads;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (c < a.d) {
+    if (g == 0 && c < a.d) {
         bf16x4 w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = (__bf16)(o[e] * inv);
-        *(bf16x4 *)(a.o + b * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
+        *(bf16x4 *)(a.o + bh / a.heads * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
     }
-    if (a.lse && c == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
+    if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
@@ -365,7 +386,7 @@ int launch_forward(const AttnFwdArgs &a, long long rows, hipStream_t st)
     hipLaunchKernelGGL((attention_kernel<D, BIAS>), dim3(work_grid(a.total)), dim3(256), lds, st, a);
     YAMD_LAUNCH_CHECK();
     if (a.splits > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<D>), dim3(ceil_div(rows * (D / 4), 256)), dim3(256), 0, st, a, rows);
+        hipLaunchKernelGGL((attention_join_kernel<D>), dim3(ceil_div(rows, 4)), dim3(256), 0, st, a, rows);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;

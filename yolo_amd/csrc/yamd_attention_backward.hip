@@ -516,19 +516,27 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         }
 }
 
-// adds the workgroups' sums by distance: thread = one distance of one head, workgroups in the order (batch, tile)
-__global__ __launch_bounds__(256) void attention_bias_grad_kernel(AttnBwdArgs a, float *dbias)
+// Adds the workgroups' sums by distance: 64 distances x 16 threads per workgroup, thread y takes every 16th of a head's
+// (tile, image) pairs and a tree in LDS adds the sixteen.
+__global__ __launch_bounds__(1024) void attention_bias_grad_kernel(AttnBwdArgs a, float *dbias)
 {
-    const int off = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
-    if (off >= a.n_off) return;
+    __shared__ float part[16][64];
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6, off = blockIdx.x * 64 + x, head = blockIdx.y;
     float s = 0.0f;
-    for (int tile = 0; tile < a.tiles; ++tile) {
+    for (int e = y; e < a.tiles * a.batch; e += 16) {
+        const int tile = e / a.batch, b = e - tile * a.batch;
         const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
         const int base = map_coord(tile * kBlockRows, a.map_w), n = map_coord(last, a.map_w) + a.coord_last - base + 1;
-        if (off < base || off - base >= n) continue;
-        for (int b = 0; b < a.batch; ++b) s += a.part_bias[(((long long)b * a.heads + head) * a.tiles + tile) * a.part_len + off - base];
+        if (off >= base && off - base < n) s += a.part_bias[(((long long)b * a.heads + head) * a.tiles + tile) * a.part_len + off - base];
     }
-    dbias[(long long)head * a.n_off + off] = s;
+    part[y][x] = s;
+    __syncthreads();
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) {
+        if (y < d) part[y][x] += part[y + d][x];
+        __syncthreads();
+    }
+    if (y == 0 && off < a.n_off) dbias[(long long)head * a.n_off + off] = part[0][x];
 }
 
 struct SumArgs {
@@ -646,7 +654,7 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
         if (rc != YAMD_OK) return rc;
     }
     if (BIAS) {
-        hipLaunchKernelGGL(attention_bias_grad_kernel, dim3(ceil_div(a.n_off, 256), a.heads), dim3(256), 0, st, w, dbias);
+        hipLaunchKernelGGL(attention_bias_grad_kernel, dim3(ceil_div(a.n_off, 64), a.heads), dim3(1024), 0, st, w, dbias);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;

@@ -27,14 +27,15 @@ template <typename T>
 struct Pack<T, 1> {
     typedef T type;
 };
+template <typename T, int VEC>
+using pack_t = typename Pack<T, VEC>::type;
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T *p, float *v)
+__device__ __forceinline__ void unpack(const pack_t<T, VEC> &t, float *v)
 {
     if constexpr (VEC == 1) {
-        v[0] = (float)*p;
+        v[0] = (float)t;
     } else {
-        const typename Pack<T, VEC>::type t = *(const typename Pack<T, VEC>::type *)p;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = (float)t[j];
     }
@@ -46,35 +47,79 @@ __device__ __forceinline__ void store_vec(T *p, const float *v)
     if constexpr (VEC == 1) {
         *p = (T)v[0];
     } else {
-        typename Pack<T, VEC>::type t;
+        pack_t<T, VEC> t;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) t[j] = (T)v[j];
-        *(typename Pack<T, VEC>::type *)p = t;
+        *(pack_t<T, VEC> *)p = t;
     }
 }
 
-// weight / bias of one vector of channels; absent ones read as `none`
-template <int VEC>
-__device__ __forceinline__ void load_param(const void *p, int bf16, int ch, float none, float *v)
+// a thread's weights or biases (parameters are aligned to their own type only); absent ones read as `none`.  at[k]: first
+// channel of its k-th vector
+template <typename P, int VEC, int VPT>
+__device__ __forceinline__ void load_params_of(const P *p, const int (&at)[VPT], float *v)
+{
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        P t[VEC];
+        __builtin_memcpy(t, p + at[k], sizeof(t));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[k * VEC + j] = (float)t[j];
+    }
+}
+template <int VEC, int VPT>
+__device__ __forceinline__ void load_params(const void *p, int bf16, const int (&at)[VPT], float none, float *v)
 {
     if (!p) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = none;
+        for (int e = 0; e < VEC * VPT; ++e) v[e] = none;
+    } else if (bf16) {
+        load_params_of<__bf16, VEC, VPT>((const __bf16 *)p, at, v);
     } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = bf16 ? (float)((const __bf16 *)p)[ch + j] : ((const float *)p)[ch + j];
+        load_params_of<float, VEC, VPT>((const float *)p, at, v);
     }
 }
 
-// sum over the TPR threads of a row, the result in all of them
+// 1 / sqrt(t): the instruction's result (1 ulp) and one Newton step; t below its range (eps = 0 only) the long way
+__device__ __forceinline__ float inverse_sqrt(float t)
+{
+    if (t < 1e-30f) return 1.0f / sqrtf(t);
+    const float r = __builtin_amdgcn_rsqf(t);
+    return r * (1.5f - 0.5f * t * r * r);
+}
+
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v)
+{
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// sum over aligned groups of W lanes, the result in all of them (register exchanges only)
+template <int W>
+__device__ __forceinline__ float lane_sum(float v)
+{
+    v = add_dpp<0xb1>(v);                      // lane ^ 1
+    v = add_dpp<0x4e>(v);                      // lane ^ 2
+    v = add_dpp<0x141>(v);                     // the other four of eight lanes
+    v = add_dpp<0x140>(v);                     // the other eight of sixteen
+    if constexpr (W >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    if constexpr (W >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    return v;
+}
+
+// sums over the TPR threads of a row, the results in all of them
 template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float *lds)
 {
     constexpr int W = TPR < 64 ? TPR : 64;
 #pragma unroll
-    for (int d = W / 2; d > 0; d >>= 1)
-#pragma unroll
-        for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], d);
+    for (int n = 0; n < N; ++n) v[n] = lane_sum<W>(v[n]);
     if constexpr (TPR > 64) {
         constexpr int NW = TPR / 64;
         const int wave = threadIdx.x >> 6;
@@ -92,6 +137,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float *lds)
     }
 }
 
+// rows that a team takes at once, so that enough loads are in flight
+template <int E, int TPR>
+constexpr int kRowsAtOnce = TPR > 256 ? 1 : E <= 8 ? 4 : 2;
+
 struct NormArgs {
     const void *x, *dy, *w, *b;
     void *y, *dx;
@@ -106,63 +155,80 @@ struct NormArgs {
 template <typename T, int VEC, int TPR, int VPT>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_kernel(NormArgs a)
 {
-    constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR, E = VEC * VPT;
-    __shared__ float lds[2 * (NT / 64)];
+    constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR, E = VEC * VPT, R = kRowsAtOnce<E, TPR>;
+    __shared__ float lds[R * (NT / 64)];
     const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const T *x = (const T *)a.x;
     T *y = (T *)a.y;
     const float inv_c = 1.0f / (float)a.c;
     float w[E], b[E];
     bool on[VPT];
+    int at[VPT];                               // a thread's vectors beyond the channels repeat the first one and count as zero
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int ch = (k * TPR + lane) * VEC;
         on[k] = ch < a.c;
-        if (on[k]) {
-            load_param<VEC>(a.w, a.param_bf16, ch, 1.0f, w + k * VEC);
-            load_param<VEC>(a.b, a.param_bf16, ch, 0.0f, b + k * VEC);
-        }
+        at[k] = on[k] ? ch : 0;
     }
-    for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows; r0 += (long long)gridDim.x * RPB) {
-        const long long r = r0 + group;
-        const bool live = r < a.rows;          // the other groups of the wave still take part in its exchanges
-        float v[E], s[1] = {0.0f};
+    load_params<VEC, VPT>(a.w, a.param_bf16, at, 1.0f, w);
+    load_params<VEC, VPT>(a.b, a.param_bf16, at, 0.0f, b);
+    for (long long r0 = (long long)blockIdx.x * RPB * R; r0 < a.rows; r0 += (long long)gridDim.x * RPB * R) {
+        // all loads first: rows beyond the last one repeat it (their teams still take part in the exchanges)
+        pack_t<T, VEC> raw[R][VPT];
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            if (live && on[k]) {
-                load_vec<T, VEC>(x + r * a.x_rs + (k * TPR + lane) * VEC, v + k * VEC);
-            } else {
+        for (int q = 0; q < R; ++q) {
+            const long long r = r0 + q * RPB + group;
+            const T *p = x + (r < a.rows ? r : a.rows - 1) * a.x_rs;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[k * VEC + j] = 0.0f;
+            for (int k = 0; k < VPT; ++k) raw[q][k] = *(const pack_t<T, VEC> *)(p + at[k]);
+        }
+        float v[R][E], mu[R], rs[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            mu[q] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                unpack<T, VEC>(raw[q][k], v[q] + k * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[q][k * VEC + j] = on[k] ? v[q][k * VEC + j] : 0.0f;
             }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[0] += v[e];
-        row_sum<TPR>(s, lds);
-        const float mu = s[0] * inv_c;
-        s[0] = 0.0f;
+        for (int q = 0; q < R; ++q)
 #pragma unroll
-        for (int k = 0; k < VPT; ++k)
+            for (int e = 0; e < E; ++e) mu[q] += v[q][e];
+        row_sum<TPR>(mu, lds);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = v[k * VEC + j] - mu;
-                v[k * VEC + j] = d;
-                s[0] += on[k] ? d * d : 0.0f;
-            }
-        row_sum<TPR>(s, lds);
-        const float rs = 1.0f / sqrtf(s[0] * inv_c + a.eps);
-        if (!live) continue;                   // TPR > 64: one group, so all threads or none
-        if (lane == 0 && a.mean) {
-            a.mean[r] = mu;
-            a.rstd[r] = rs;
+        for (int q = 0; q < R; ++q) {
+            mu[q] *= inv_c;
+            rs[q] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < VPT; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float d = v[q][k * VEC + j] - mu[q];
+                    v[q][k * VEC + j] = d;
+                    rs[q] += on[k] ? d * d : 0.0f;
+                }
         }
+        row_sum<TPR>(rs, lds);
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            if (!on[k]) continue;
-            float o[VEC];
+        for (int q = 0; q < R; ++q) {
+            const long long r = r0 + q * RPB + group;
+            if (r >= a.rows) continue;
+            const float s = inverse_sqrt(rs[q] * inv_c + a.eps);
+            if (lane == 0 && a.mean) {
+                a.mean[r] = mu[q];
+                a.rstd[r] = s;
+            }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = v[k * VEC + j] * rs * w[k * VEC + j] + b[k * VEC + j];
-            store_vec<T, VEC>(y + r * a.y_rs + (k * TPR + lane) * VEC, o);
+            for (int k = 0; k < VPT; ++k) {
+                if (!on[k]) continue;
+                float o[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o[j] = v[q][k * VEC + j] * s * w[k * VEC + j] + b[k * VEC + j];
+                store_vec<T, VEC>(y + r * a.y_rs + (k * TPR + lane) * VEC, o);
+            }
         }
     }
 }
@@ -170,8 +236,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_kernel(NormA
 template <typename T, int VEC, int TPR, int VPT>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_backward_kernel(NormArgs a)
 {
-    constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR, E = VEC * VPT;
-    __shared__ float lds[2 * (NT / 64)];
+    constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR, E = VEC * VPT, R = E <= 8 ? 2 : 1;
+    __shared__ float lds[2 * R * (NT / 64)];
     __shared__ float acc[RPB > 1 ? 2 * TPR * E : 1];
     const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const T *x = (const T *)a.x, *dy = (const T *)a.dy;
@@ -179,49 +245,72 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_backward_ker
     const float inv_c = 1.0f / (float)a.c;
     float w[E], dw[E], db[E];
     bool on[VPT];
+    int at[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int ch = (k * TPR + lane) * VEC;
         on[k] = ch < a.c;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) w[k * VEC + j] = dw[k * VEC + j] = db[k * VEC + j] = 0.0f;
-        if (on[k]) load_param<VEC>(a.w, a.param_bf16, ch, 1.0f, w + k * VEC);
+        at[k] = on[k] ? ch : 0;
     }
-    for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows; r0 += (long long)gridDim.x * RPB) {
-        const long long r = r0 + group;
-        const bool live = r < a.rows;
-        float xh[E], g[E], s[2] = {0.0f, 0.0f};
-        const float mu = live ? a.mean_in[r] : 0.0f, rs = live ? a.rstd_in[r] : 0.0f;
+    load_params<VEC, VPT>(a.w, a.param_bf16, at, 1.0f, w);
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            if (live && on[k]) {
-                load_vec<T, VEC>(x + r * a.x_rs + (k * TPR + lane) * VEC, xh + k * VEC);
-                load_vec<T, VEC>(dy + r * a.dy_rs + (k * TPR + lane) * VEC, g + k * VEC);
-            } else {
+    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
+    for (long long r0 = (long long)blockIdx.x * RPB * R; r0 < a.rows; r0 += (long long)gridDim.x * RPB * R) {
+        pack_t<T, VEC> raw_x[R][VPT], raw_g[R][VPT];
+        float xh[R][E], g[R][E], mu[R], rs[R], s[2 * R];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) xh[k * VEC + j] = mu, g[k * VEC + j] = 0.0f;
+        for (int q = 0; q < R; ++q) {
+            const long long r = r0 + q * RPB + group, rr = r < a.rows ? r : a.rows - 1;
+            mu[q] = a.mean_in[rr];
+            rs[q] = a.rstd_in[rr];
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                raw_x[q][k] = *(const pack_t<T, VEC> *)(x + rr * a.x_rs + at[k]);
+                raw_g[q][k] = *(const pack_t<T, VEC> *)(dy + rr * a.dy_rs + at[k]);
             }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            xh[e] = (xh[e] - mu) * rs;
-            dw[e] += g[e] * xh[e];
-            db[e] += g[e];
-            g[e] *= w[e];
-            s[0] += g[e];
-            s[1] += g[e] * xh[e];
+        for (int q = 0; q < R; ++q) {
+            const bool live = r0 + q * RPB + group < a.rows;
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                unpack<T, VEC>(raw_x[q][k], xh[q] + k * VEC);
+                unpack<T, VEC>(raw_g[q][k], g[q] + k * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    xh[q][k * VEC + j] = live && on[k] ? xh[q][k * VEC + j] : mu[q];
+                    g[q][k * VEC + j] = live && on[k] ? g[q][k * VEC + j] : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            s[2 * q] = s[2 * q + 1] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                xh[q][e] = (xh[q][e] - mu[q]) * rs[q];
+                dw[e] += g[q][e] * xh[q][e];
+                db[e] += g[q][e];
+                g[q][e] *= w[e];
+                s[2 * q] += g[q][e];
+                s[2 * q + 1] += g[q][e] * xh[q][e];
+            }
         }
         if (!a.dx) continue;
         row_sum<TPR>(s, lds);
-        if (!live) continue;
-        const float m0 = s[0] * inv_c, m1 = s[1] * inv_c;
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            if (!on[k]) continue;
-            float o[VEC];
+        for (int q = 0; q < R; ++q) {
+            const long long r = r0 + q * RPB + group;
+            if (r >= a.rows) continue;
+            const float m0 = s[2 * q] * inv_c, m1 = s[2 * q + 1] * inv_c;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = rs * (g[k * VEC + j] - m0 - xh[k * VEC + j] * m1);
-            store_vec<T, VEC>(dx + r * a.dx_rs + (k * TPR + lane) * VEC, o);
+            for (int k = 0; k < VPT; ++k) {
+                if (!on[k]) continue;
+                float o[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o[j] = rs[q] * (g[q][k * VEC + j] - m0 - xh[q][k * VEC + j] * m1);
+                store_vec<T, VEC>(dx + r * a.dx_rs + (k * TPR + lane) * VEC, o);
+            }
         }
     }
     if (!a.partial) return;
@@ -374,7 +463,7 @@ extern "C" int yamd_layer_norm(const void *x, long long x_stride, const void *we
     const int vec = wide ? v : 1;
     const Team t = team_for(c, vec);
     const long long rpb = t.tpr > 256 ? 1 : 256 / t.tpr;
-    const long long want = (rows + rpb - 1) / rpb, most = 256 * (t.tpr > 256 ? 2 : 8);
+    const long long want = (rows + rpb - 1) / rpb, most = 256 * (t.tpr > 256 ? 2 : 8);     // (more than the rounds need: they end at once)
     const int blocks = (int)(want < most ? want : most);
     if (dtype == YAMD_BF16) dispatch<__bf16>(false, a, vec, blocks, (hipStream_t)stream);
     else dispatch<float>(false, a, vec, blocks, (hipStream_t)stream);
