@@ -30,7 +30,8 @@ struct AttnView {
 template <int D>
 struct Tile {
     static constexpr int kChunks = D <= 32 ? 4 : D <= 64 ? 8 : 16;      // per row; D = 96 leaves the last four unused
-    static constexpr int kRowBytes = kChunks * 16, kBytes = kTile * kRowBytes;
+    static constexpr int kRowBytes = kChunks * 16;
+    static constexpr int bytes(int rows) { return rows * kRowBytes; }
     __device__ static __forceinline__ int swizzle(int r)
     {
         if constexpr (kChunks == 4) return (r >> 2) & 3;
@@ -51,40 +52,49 @@ __device__ __forceinline__ f32x16 zero16()
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-// A operand of rows [row0, row0 + 32) of a tile, columns 16 ks .. 16 ks + 15
-template <int D>
-__device__ __forceinline__ bf16x8 rows_operand(const char *tile, int row0, int ks, int lane)
-{
-    using T = Tile<D>;
-    const int r = lane & 31;
-    return *(const bf16x8 *)(tile + row0 * T::kRowBytes + r * T::kRowBytes + (((2 * ks + (lane >> 5)) ^ T::swizzle(r)) << 4));
-}
-
 __device__ __forceinline__ s16x4 transposed_quad(const char *at)
 {
     typedef __attribute__((address_space(3))) s16x4 lds_quad;
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad *)at);
 }
 
-// A operand of the transposed tile: rows are the tile's columns col0 .. col0 + 31, k slots its rows in the order that the
-// accumulator rows 16 u .. 16 u + 15 (counted from row0) have as a B operand.  Each group of 16 lanes reads 4 rows of 16
-// columns and gets them transposed: lane i of the group gives the address of row i / 4, columns 4 (i % 4) .. + 3 and
-// receives the 4 rows of column i.
+// Where a lane reads a tile.  Columns enter a swizzled address as an exclusive or, so one lane constant serves each kind of
+// operand: `row` for 16 bytes of row (lane & 31), `quad` for the transposing reads.
 template <int D>
-__device__ __forceinline__ bf16x8 transposed_operand(const char *tile, int row0, int col0, int lane)
-{
+struct TileReader {
     using T = Tile<D>;
-    const int i = lane & 15, g = lane >> 4;
-    const int r = 4 * (g >> 1) + (i >> 2), c = col0 / 8 + 2 * (g & 1) + ((i >> 1) & 1);
-    const char *base = tile + row0 * T::kRowBytes + (i & 1) * 8;
-    union {
-        s16x4 q[2];
-        bf16x8 v;
-    } o;
-    o.q[0] = transposed_quad(base + r * T::kRowBytes + ((c ^ T::swizzle(r)) << 4));
-    o.q[1] = transposed_quad(base + (r + 8) * T::kRowBytes + ((c ^ T::swizzle(r + 8)) << 4));
-    return o.v;
-}
+    unsigned row, quad;
+
+    __device__ __forceinline__ explicit TileReader(int lane)
+    {
+        const int r = lane & 31, i = lane & 15, g = lane >> 4, rq = 4 * (g >> 1) + (i >> 2);
+        row = r * T::kRowBytes + (((lane >> 5) ^ T::swizzle(r)) << 4);
+        quad = rq * T::kRowBytes + (((2 * (g & 1) + ((i >> 1) & 1)) ^ T::swizzle(rq)) << 4) + (i & 1) * 8;
+    }
+    // hides the constants' origin: the addresses made from them are then computed where they are used instead of being kept
+    // in registers across the loop, of which wide heads have none to spare
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(row), "+v"(quad)); }
+
+    // A (or B) operand of rows [row0, row0 + 32), columns 16 ks .. 16 ks + 15
+    __device__ __forceinline__ bf16x8 rows(const char *tile, int row0, int ks) const
+    {
+        return *(const bf16x8 *)(tile + row0 * T::kRowBytes + (row ^ (ks << 5)));
+    }
+    // A operand of the transposed tile: rows are the tile's columns 32 n .. 32 n + 31, k slots its rows in the order that the
+    // accumulator rows 0 .. 15 (counted from row0) have as a B operand.  Each group of 16 lanes reads 4 rows of 16 columns and
+    // gets them transposed: lane i of the group gives the address of row i / 4, columns 4 (i % 4) .. + 3 and receives the
+    // 4 rows of column i.
+    __device__ __forceinline__ bf16x8 transposed(const char *tile, int row0, int n) const
+    {
+        union {
+            s16x4 q[2];
+            bf16x8 v;
+        } o;
+        o.q[0] = transposed_quad(tile + row0 * T::kRowBytes + (quad ^ (n << 6)));
+        o.q[1] = transposed_quad(tile + (row0 + 8) * T::kRowBytes + (quad ^ (n << 6) ^ 32));      // swizzle(r + 8) = swizzle(r) ^ 2
+        return o.v;
+    }
+};
 
 // B operand from eight consecutive accumulator values
 __device__ __forceinline__ bf16x8 acc_operand(const f32x16 &v, int u)
@@ -136,10 +146,11 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 
 // Fills tiles with rows of a token axis of `len` rows (256 threads, each wave a quarter).  Rows beyond the axis repeat its
 // last row, chunks beyond the head width d are left as they are: both are cleared by the caller.
-template <int D>
+template <int D, int ROWS = kTile>
 struct TileLoader {
     using T = Tile<D>;
-    static constexpr int N = T::kChunks / 4;
+    static constexpr int N = T::kChunks * ROWS / 256;
+    static_assert(N * 256 == T::kChunks * ROWS, "every thread moves whole pieces");
     unsigned offset[N];            // of this lane's pieces of a whole tile
     unsigned row_bytes;
     bool on[N];
@@ -160,7 +171,7 @@ struct TileLoader {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             unsigned o = offset[n];
-            if (last < kTile - 1) {
+            if (last < ROWS - 1) {
                 const int r = ((n * 4 + wave) * 64 + lane) / T::kChunks;
                 o -= (r > last ? r - last : 0) * row_bytes;
             }
@@ -176,12 +187,12 @@ __device__ __forceinline__ void clear_lds(char *p, int bytes)
 }
 
 // zeros in the rows whose bit of `keep` is clear: four threads per row
-template <int D>
+template <int D, int ROWS = kTile>
 __device__ __forceinline__ void clear_rows(char *tile, unsigned long long keep)
 {
     using T = Tile<D>;
     const int r = threadIdx.x >> 2;
-    if ((keep >> r) & 1) return;
+    if (r >= ROWS || ((keep >> r) & 1)) return;
 #pragma unroll
     for (int c = 0; c < T::kChunks / 4; ++c) *(uint4 *)(tile + r * T::kRowBytes + ((threadIdx.x & 3) * (T::kChunks / 4) + c) * 16) = make_uint4(0, 0, 0, 0);
 }

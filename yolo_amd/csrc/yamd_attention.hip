@@ -35,7 +35,7 @@ struct AttnFwdArgs {
 // windows of the bias
 template <int D>
 struct FwdLds {
-    static constexpr int K = Tile<D>::kBytes, BUF = 2 * K, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
+    static constexpr int K = Tile<D>::bytes(kTile), BUF = 2 * K, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
     static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 : 0); }
 };
 
@@ -109,7 +109,9 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
     // (a wait that the compiler sees: it would otherwise wait for the query rows inside the loop, and for the tiles with them)
     __builtin_amdgcn_s_waitcnt(0x0f70);
     if (t0 < t1) fetch(t0);
+    TileReader<D> reader(lane);
     for (int t = t0; t < t1; ++t) {
+        if constexpr (D > 64) reader.forget();
         char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::K;
         int *const coord = (int *)(smem + L::COORD) + (t & 1) * kTile;
         unsigned long long *const kept = (unsigned long long *)(smem + L::KEEP) + (t & 1);
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) kf[u][ks] = rows_operand<D>(kt, 32 * u, ks, lane);
+            for (int ks = 0; ks < NKS; ++ks) kf[u][ks] = reader.rows(kt, 32 * u, ks);
         float bias_of[BIAS ? 32 : 1];
         if constexpr (BIAS) {
             const float *const w = (const float *)(smem + L::WINDOW) + (t & 1) * a.window + (c_row - window_from(t));
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int n = 0; n < NB; ++n) f[u][n] = transposed_operand<D>(vt, from + 16 * u, 32 * n, lane);
+                for (int n = 0; n < NB; ++n) f[u][n] = reader.transposed(vt, from + 16 * u, n);
         };
         if constexpr (EARLY) read_values(vf, 0);
         if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);

@@ -63,18 +63,23 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
 // ---- dk, dv ------------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys (the result's columns); tiles of 64 queries pass through LDS.  S = Q K^T and dP = dO V^T read the
 // tile's rows, dV^T += dO^T P and dK^T += Q^T dS read it transposed.
+// Wide heads (D > 64) have no registers for the values beside the keys and both results: their values stay in LDS, and the
+// tiles are 32 queries so that two workgroups share a CU.
 template <int D>
 struct KvLds {
-    static constexpr int T = Tile<D>::kBytes, BUF = 2 * T, STATS = 2 * BUF, WINDOW = STATS + 2 * 3 * kTile * 4;
+    static constexpr int ROWS = D <= 64 ? kTile : 32;
+    static constexpr bool VALUES = D > 64;
+    static constexpr int T = Tile<D>::bytes(ROWS), BUF = 2 * T, V = 2 * BUF, STATS = V + (VALUES ? Tile<D>::bytes(kBlockRows) : 0);
+    static constexpr int WINDOW = STATS + 2 * 3 * ROWS * 4;
     static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 : 0); }
 };
 
 template <int D, bool BIAS>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(AttnBwdArgs a)
+__global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
 {
     using L = KvLds<D>;
-    constexpr int NKS = D / 16, NB = D / 32;
-    constexpr bool EARLY = true;                    // wider heads have no registers left to request operands ahead
+    constexpr int NKS = D / 16, NB = D / 32, ROWS = L::ROWS;
+    constexpr bool EARLY = D <= 64;                    // wider heads have no registers left to request operands ahead
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
     int item = work_item();
@@ -91,7 +96,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
     const bool valid = key0 + c32 < a.k_len && (!a.mask || a.mask[b * a.mask_sb + key] != 0);
     const bool busy = __any(valid);
 
-    bf16x8 kf[NKS], vf[NKS];
+    bf16x8 kf[NKS], vf[L::VALUES ? 1 : NKS];
     {
         const __bf16 *kp = a.k.p + b * a.k.sb + (long long)key * a.k.st + kv_head * a.k.sh;
         const __bf16 *vp = a.v.p + b * a.v.sb + (long long)key * a.v.st + kv_head * a.v.sh;
@@ -100,10 +105,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
             const int c = 16 * ks + 8 * half;
             if (valid && c < a.d) {
                 kf[ks] = *(const bf16x8 *)(kp + c);
-                vf[ks] = *(const bf16x8 *)(vp + c);
+                if constexpr (!L::VALUES) vf[ks] = *(const bf16x8 *)(vp + c);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) kf[ks][e] = vf[ks][e] = (__bf16)0.0f;
+                for (int e = 0; e < 8; ++e) {
+                    kf[ks][e] = (__bf16)0.0f;
+                    if constexpr (!L::VALUES) vf[ks][e] = (__bf16)0.0f;
+                }
             }
         }
     }
@@ -118,12 +126,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
     const float c2 = a.scale * kLog2e, inv_scale = 1.0f / a.scale;
 
     // the loop runs over (head of the group, tile of queries)
-    const int q_tiles = (a.q_len + kTile - 1) / kTile, loop = a.group * q_tiles;
+    const int q_tiles = (a.q_len + ROWS - 1) / ROWS, loop = a.group * q_tiles;
     const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < loop ? t0 + a.loop_per_split : loop;
-    const TileLoader<D> ql(a.q.st, a.d, wave, lane), gl(a.go.st, a.d, wave, lane);
+    const TileLoader<D, ROWS> ql(a.q.st, a.d, wave, lane), gl(a.go.st, a.d, wave, lane);
     float lse_n = 0.0f, delta_n = 0.0f;
     auto fetch = [&](int t) {
-        const int head = kv_head * a.group + t / q_tiles, first = t % q_tiles * kTile;
+        const int head = kv_head * a.group + t / q_tiles, first = t % q_tiles * ROWS;
         char *const qt = smem + (t & 1) * L::BUF;
         ql.load(qt, a.q.p + b * a.q.sb + head * a.q.sh, first, a.q_len, wave, lane);
         gl.load(qt + L::T, a.go.p + b * a.go.sb + head * a.go.sh, first, a.q_len, wave, lane);
@@ -134,7 +142,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
             // rows beyond the queries, and rows without keys, get an infinite sum: their probabilities are exp2(-inf) = 0
             lse_n = INFINITY;
             delta_n = 0.0f;
-            if (first + lane < a.q_len) {
+            if (lane < ROWS && first + lane < a.q_len) {
                 const long long w = ((long long)b * a.heads + head) * a.q_len + first + lane;
                 lse_n = a.lse[w];
                 delta_n = a.delta[w];
@@ -142,46 +150,52 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
         }
     };
     if (a.d < D) {                                     // channels beyond the head width: zeros that no load overwrites
-        clear_lds(smem, 2 * L::BUF);
+        clear_lds(smem, L::STATS);
         __syncthreads();
+    }
+    if constexpr (L::VALUES) {
+        const TileLoader<D, kBlockRows> vl(a.v.st, a.d, wave, lane);
+        vl.load(smem + L::V, a.v.p + b * a.v.sb + kv_head * a.v.sh, tile * kBlockRows, a.k_len, wave, lane);
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     if (t0 < t1) fetch(t0);
+    TileReader<D> reader(lane);
     for (int t = t0; t < t1; ++t) {
+        if constexpr (D > 64) reader.forget();
         char *const qt = smem + (t & 1) * L::BUF, *const gt = qt + L::T;
-        float *const lse_s = (float *)(smem + L::STATS) + (t & 1) * 3 * kTile, *const delta = lse_s + kTile;
-        int *const coord = (int *)(delta + kTile);
-        if (wave == 0) {
+        float *const lse_s = (float *)(smem + L::STATS) + (t & 1) * 3 * ROWS, *const delta = lse_s + ROWS;
+        int *const coord = (int *)(delta + ROWS);
+        if (wave == 0 && lane < ROWS) {
             lse_s[lane] = lse_n == -INFINITY ? -INFINITY : -lse_n * inv_scale;
             delta[lane] = -delta_n;
         }
-        if (BIAS && tid < kTile) {
-            const int i = t % q_tiles * kTile + tid;
+        if (BIAS && tid < ROWS) {
+            const int i = t % q_tiles * ROWS + tid;
             coord[tid] = map_coord(i < a.q_len ? i : a.q_len - 1, a.map_w);
         }
         landed();
         __syncthreads();
         // read from LDS by all waves, so that they agree on the barrier below
-        const unsigned long long keep = uniform64(__ballot(lse_s[lane] != -INFINITY));
+        const unsigned long long keep = uniform64(__ballot(lane >= ROWS || lse_s[lane & (ROWS - 1)] != -INFINITY));
         if (t + 1 < t1) fetch(t + 1);
         if (keep != ~0ull) {                           // a row without keys gives no gradient whatever q and do hold
-            clear_rows<D>(qt, keep);
-            clear_rows<D>(gt, keep);
+            clear_rows<D, ROWS>(qt, keep);
+            clear_rows<D, ROWS>(gt, keep);
             __syncthreads();
         }
         const float *const win = (const float *)(smem + L::WINDOW) + (t & 1) * a.window +
-                                 (BIAS ? c_key - c_low - map_coord(t % q_tiles * kTile, a.map_w) : 0);
+                                 (BIAS ? c_key - c_low - map_coord(t % q_tiles * ROWS, a.map_w) : 0);
         if (!busy) continue;
         // Operands are requested one stage ahead of the products that use them, as far as registers allow; fences keep the
         // scheduler from putting each read right before its product.  Columns (keys) do not mix, so a masked key's column
         // may hold anything until its result is replaced by zeros at the end.
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < ROWS / 32; ++u) {
             bf16x8 qr[NKS], gr[NKS];
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) qr[ks] = rows_operand<D>(qt, 32 * u, ks, lane);
+            for (int ks = 0; ks < NKS; ++ks) qr[ks] = reader.rows(qt, 32 * u, ks);
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) gr[ks] = rows_operand<D>(gt, 32 * u, ks, lane);
+            for (int ks = 0; ks < NKS; ++ks) gr[ks] = reader.rows(gt, 32 * u, ks);
             // both products start from a row's statistics: s from -lse / scale, dP from -D
             f32x16 s, g;
             int at[BIAS ? 16 : 1];
@@ -200,14 +214,17 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) s = mfma(qr[ks], kf[ks], s);
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) g = mfma(gr[ks], vf[ks], g);
+            for (int ks = 0; ks < NKS; ++ks) {
+                if constexpr (L::VALUES) g = mfma(gr[ks], reader.rows(smem + L::V, 32 * wave, ks), g);
+                else g = mfma(gr[ks], vf[ks], g);
+            }
             bf16x8 gx[2][NB], qx[2][NB];
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    gx[w][n] = transposed_operand<D>(gt, 32 * u + 16 * w, 32 * n, lane);
-                    qx[w][n] = transposed_operand<D>(qt, 32 * u + 16 * w, 32 * n, lane);
+                    gx[w][n] = reader.transposed(gt, 32 * u + 16 * w, n);
+                    qx[w][n] = reader.transposed(qt, 32 * u + 16 * w, n);
                 }
             if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -273,7 +290,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_dkv_kernel(Att
 // 2 * 127 + 1 positions, and where a map has several rows 127 + 127 + 2 w more.
 template <int D>
 struct QLds {
-    static constexpr int T = Tile<D>::kBytes, BUF = 2 * T, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
+    static constexpr int T = Tile<D>::bytes(kTile), BUF = 2 * T, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
     static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 + 8 * (2048 + kRingPad) * 4 : 0); }
 };
 
@@ -377,7 +394,9 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     if (t0 < t1) fetch(t0);
+    TileReader<D> reader(lane);
     for (int t = t0; t < t1; ++t) {
+        if constexpr (D > 64) reader.forget();
         char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::T;
         int *const coord = (int *)(smem + L::COORD) + (t & 1) * kTile;
         unsigned long long *const kept = (unsigned long long *)(smem + L::KEEP) + (t & 1);
@@ -418,8 +437,8 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int ks = 0; ks < NKS; ++ks) {
-                    kr[u][ks] = rows_operand<D>(kt, 32 * u, ks, lane);
-                    vr[u][ks] = rows_operand<D>(vt, 32 * u, ks, lane);
+                    kr[u][ks] = reader.rows(kt, 32 * u, ks);
+                    vr[u][ks] = reader.rows(vt, 32 * u, ks);
                 }
             __builtin_amdgcn_sched_barrier(0);
             f32x16 s[2], g[2];
@@ -435,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 #pragma unroll
             for (int w = 0; w < 4; ++w)
 #pragma unroll
-                for (int n = 0; n < NB; ++n) kx[w][n] = transposed_operand<D>(kt, 16 * w, 32 * n, lane);
+                for (int n = 0; n < NB; ++n) kx[w][n] = reader.transposed(kt, 16 * w, n);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -466,9 +485,9 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
             for (int u = 0; u < 2; ++u) {
                 f32x16 s = zero16(), g = zero16();
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) s = mfma(rows_operand<D>(kt, 32 * u, ks, lane), qf[ks], s);
+                for (int ks = 0; ks < NKS; ++ks) s = mfma(reader.rows(kt, 32 * u, ks), qf[ks], s);
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) g = mfma(rows_operand<D>(vt, 32 * u, ks, lane), gf[ks], g);
+                for (int ks = 0; ks < NKS; ++ks) g = mfma(reader.rows(vt, 32 * u, ks), gf[ks], g);
                 score_gradient(s, g, u);
                 if constexpr (BIAS) {
 #pragma unroll
@@ -481,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
                 for (int w = 0; w < 2; ++w) {
                     const bf16x8 sf = acc_operand(g, w);
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) dq[n] = mfma(transposed_operand<D>(kt, 32 * u + 16 * w, 32 * n, lane), sf, dq[n]);
+                    for (int n = 0; n < NB; ++n) dq[n] = mfma(reader.transposed(kt, 32 * u + 16 * w, n), sf, dq[n]);
                 }
             }
         }
@@ -589,7 +608,7 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     BwdPlan p = {};
     p.dpad = padded_head_dim(d->head_dim);
     const long long bh = (long long)d->batch * d->heads, bk = (long long)d->batch * d->kv_heads;
-    const int kt = ceil_div(d->k_len, kTile), qt = ceil_div(d->q_len, kTile) * (d->heads / d->kv_heads);
+    const int kt = ceil_div(d->k_len, kTile), qt = ceil_div(d->q_len, p.dpad <= 64 ? kTile : 32) * (d->heads / d->kv_heads);
     p.kv_tiles = ceil_div(d->k_len, kBlockRows);
     p.q_tiles = ceil_div(d->q_len, kBlockRows);
     const long long kw = bk * p.kv_tiles, qw = bh * p.q_tiles;
