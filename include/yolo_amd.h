@@ -400,7 +400,7 @@ typedef struct yamd_attention_desc {
     int32_t batch, heads, kv_heads;     /* heads % kv_heads == 0: consecutive heads share a key / value head */
     int32_t head_dim;                   /* multiple of 8, at most 128 */
     int32_t q_len, k_len;
-    int32_t map_h, map_w;               /* with a bias: q_len == k_len == map_h * map_w, map_w <= 768 unless map_h == 1 */
+    int32_t map_h, map_w;               /* with a bias: q_len == k_len == map_h * map_w, map_w <= 760 unless map_h == 1 */
     float scale;                        /* > 0 */
 } yamd_attention_desc;
 
@@ -409,18 +409,20 @@ typedef struct yamd_attention_desc {
  *             there does not matter.  A query that is left without keys gets zeros.
  *   bias      (heads rows of (2 map_h - 1)(2 map_w - 1) floats; NULL = none): added to the score of a query at (y, x) and a
  *             key at (y', x') from [(y - y' + map_h - 1)(2 map_w - 1) + x - x' + map_w - 1].
+ *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted; only with a bias): o before its
+ *             rounding to bf16 and with probabilities kept to 16 bits, which the gradient of a bias needs.
  *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
  * The workspace (16-byte aligned; 0 bytes for most shapes) holds parts of o where the keys are split over workgroups. */
 size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biased);
 int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
-                   const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, float *lse,
-                   void *workspace, size_t workspace_bytes, void *stream);
+                   const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,
+                   float *o_exact, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* Gradients of the above from o, lse and d_o; the probabilities are computed again.  dbias: one float per head and distance
- * (given exactly when bias is).  Every sum is taken in a fixed order: equal inputs give equal bits. */
+ * (NULL: the bias has no gradient; otherwise o_exact is needed too).  Every sum is taken in a fixed order: equal inputs give equal bits. */
 size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *desc, int biased);
 int yamd_attention_backward(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
-                            const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, const float *lse,
-                            const yamd_tokens *d_o, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv, float *dbias,
+                            const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, const float *o_exact,
+                            const float *lse, const yamd_tokens *d_o, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv, float *dbias,
                             void *workspace, size_t workspace_bytes, void *stream);
 
 /* A position bias learned by buckets of distance: bias[head][i] = table[bucket_of[i]][head] for n_distances distances (a

@@ -226,7 +226,33 @@ __device__ __forceinline__ void load_window(char *lds, const float *bias, int fr
         load_lds_4(bias, (o < 0 ? 0 : o < n_off ? o : n_off - 1) * 4u, lds + at * 4);
     }
 }
+// Forms of the bias.  In quads (a sequence, or a map whose width is a multiple of 4) four tokens from a multiple of 4 on
+// lie next to each other, so one coordinate serves four rows of an accumulator.
+enum Bias { kNoBias, kAnyBias, kQuadBias };
+
+// the biases of a lane's sixteen accumulator rows: win[coord] (SIGN = 1) or win[-coord] for rows 32 u + acc_row(r, half)
+template <int BIAS, int SIGN>
+__device__ __forceinline__ void read_bias(float (&b)[16], const float *win, const int *coord, int u, int half)
+{
+    if constexpr (BIAS == kQuadBias) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = coord[32 * u + acc_row(4 * g, half)];
+            const float *const p = SIGN > 0 ? win + c : win - c - 3;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[4 * g + j] = p[SIGN > 0 ? j : 3 - j];
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) b[r] = win[SIGN * coord[32 * u + acc_row(r, half)]];
+    }
+}
+
 // distances between 128 owned rows and a tile of 64, rounded up to what four waves load at once
+static inline Bias bias_form(const float *bias, int map_h, int map_w)
+{
+    return !bias ? kNoBias : map_h == 1 || map_w % 4 == 0 ? kQuadBias : kAnyBias;
+}
 static inline int window_len(int map_h, int map_w)
 {
     const int n = kBlockRows + kTile + (map_h > 1 ? kBlockRows + kTile + 2 * map_w : 0);

@@ -8,6 +8,10 @@
 // Probabilities are rounded to bf16 for the second product only (their sum is taken before, in float32): the error of o is
 // at most 2^-8 of the weighted mean of |v|, below the rounding of o itself in all but contrived cases.
 //
+// Where the bias has a gradient, the backward pass needs o more exactly than that (yamd_attention_backward.hip): with
+// o_exact the second product runs twice, for the probabilities rounded to bf16 and for what the rounding left (2^-17 of them
+// is lost), and o is also written in float32.
+//
 // Few query rows: heads that share keys are packed into one tile of rows (row = head in group * q_len + query), and the
 // keys are split over workgroups whose float32 parts a second kernel joins.
 #include "yamd_attention.h"
@@ -20,6 +24,7 @@ struct AttnFwdArgs {
     AttnView q, k, v;
     __bf16 *o;
     long long o_sb, o_st, o_sh;
+    float *o_exact;                // [batch][heads][q_len][d], o before rounding, or null (see below)
     float *lse;                    // [batch][heads][q_len], natural logarithm, or null
     const uint8_t *mask;           // [batch][k_len], 0 = not attended, or null
     long long mask_sb;
@@ -39,7 +44,7 @@ struct FwdLds {
     static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 : 0); }
 };
 
-template <int D, bool BIAS>
+template <int D, int BIAS, bool EXACT>
 __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
 {
     using L = FwdLds<D>;
@@ -89,10 +94,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
     const float *bias = BIAS ? a.bias + (long long)gh * a.n_off : nullptr;
     const int c_row = BIAS ? a.coord_last + map_coord(i, a.map_w) : 0;
     const int c_first = BIAS ? a.coord_last + map_coord(q_tile * kBlockRows, a.map_w) : 0;
-    auto window_from = [&](int t) {
-        const int last = t * kTile + kTile - 1;
-        return c_first - map_coord(last < a.k_len ? last : a.k_len - 1, a.map_w);
-    };
+    auto window_from = [&](int t) { return c_first - map_coord(t * kTile + kTile - 1, a.map_w); };
     const TileLoader<D> kl(a.k.st, a.d, wave, lane), vl(a.v.st, a.d, wave, lane);
     unsigned char mask_n = 1;
     auto fetch = [&](int t) {
@@ -115,10 +117,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         char *const kt = smem + (t & 1) * L::BUF, *const vt = kt + L::K;
         int *const coord = (int *)(smem + L::COORD) + (t & 1) * kTile;
         unsigned long long *const kept = (unsigned long long *)(smem + L::KEEP) + (t & 1);
-        if (BIAS && tid < kTile) {
-            const int key = t * kTile + tid;
-            coord[tid] = map_coord(key < a.k_len ? key : a.k_len - 1, a.map_w);
-        }
+        if (BIAS && tid < kTile) coord[tid] = map_coord(t * kTile + tid, a.map_w);       // (keys beyond the last one continue)
         if (mp && wave == 0) {
             const unsigned long long v = __ballot(mask_n != 0);
             if (lane == 0) *kept = v;
@@ -148,11 +147,11 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) kf[u][ks] = reader.rows(kt, 32 * u, ks);
-        float bias_of[BIAS ? 32 : 1];
+        float bias_of[2][16];
         if constexpr (BIAS) {
             const float *const w = (const float *)(smem + L::WINDOW) + (t & 1) * a.window + (c_row - window_from(t));
-#pragma unroll
-            for (int r = 0; r < 32; ++r) bias_of[r] = w[-coord[32 * (r >> 4) + acc_row(r & 15, half)]];
+            read_bias<BIAS, -1>(bias_of[0], w, coord, 0, half);
+            read_bias<BIAS, -1>(bias_of[1], w, coord, 1, half);
         }
         if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -172,7 +171,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
         if constexpr (BIAS) {
 #pragma unroll
-            for (int r = 0; r < 32; ++r) s[r >> 4][r & 15] = __builtin_fmaf(s[r >> 4][r & 15], a.scale, bias_of[r]);
+            for (int r = 0; r < 32; ++r) s[r >> 4][r & 15] = __builtin_fmaf(s[r >> 4][r & 15], a.scale, bias_of[r >> 4][r & 15]);
         }
         if (keep != ~0ull) {
             mask_rows(s[0], keep, 0, half);
@@ -208,19 +207,24 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         if constexpr (EARLY) read_values(vg, 32);
         else read_values(vf, 0);
         if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+        auto add_values = [&](const f32x16 &p, const bf16x8 (&f)[2][NB]) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const bf16x8 pf = acc_operand(s[0], u);
+            for (int u = 0; u < 2; ++u) {
+                const bf16x8 pf = acc_operand(p, u);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) acc[n] = mfma(vf[u][n], pf, acc[n]);
-        }
+                for (int n = 0; n < NB; ++n) acc[n] = mfma(f[u][n], pf, acc[n]);
+                if constexpr (EXACT) {
+                    bf16x8 rest;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) rest[e] = (__bf16)(p[8 * u + e] - (float)pf[e]);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) acc[n] = mfma(f[u][n], rest, acc[n]);
+                }
+            }
+        };
+        add_values(s[0], vf);
         if constexpr (!EARLY) read_values(vg, 32);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const bf16x8 pf = acc_operand(s[1], u);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) acc[n] = mfma(vg[u][n], pf, acc[n]);
-        }
+        add_values(s[1], vg);
     }
     l = with_other_half(l, [](float x, float y) { return x + y; });
     if (row0 + c32 >= a.rows) return;
@@ -245,9 +249,14 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
             const int c = 32 * n + 8 * g + 4 * half;
             if (c < a.d) {
                 bf16x4 o;
+                f32x4 x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (__bf16)(acc[n][4 * g + e] * inv);
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = acc[n][4 * g + e] * inv;
+                    o[e] = (__bf16)x[e];
+                }
                 *(bf16x4 *)(op + c) = o;
+                if constexpr (EXACT) *(f32x4 *)(a.o_exact + (((long long)b * a.heads + head) * a.q_len + i) * a.d + c) = x;
             }
         }
     if (a.lse && half == 0)
@@ -302,8 +311,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (g == 0 && c < a.d) {
         bf16x4 w;
+        o *= inv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = (__bf16)(o[e] * inv);
+        for (int e = 0; e < 4; ++e) w[e] = (__bf16)o[e];
+        if (a.o_exact) *(f32x4 *)(a.o_exact + at * a.d + c) = o;
         *(bf16x4 *)(a.o + bh / a.heads * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
     }
     if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
@@ -326,7 +337,7 @@ int check_attention(const yamd_attention_desc *d, const uint8_t *key_mask, long 
         YAMD_REQUIRE(d->map_h > 0 && d->map_w > 0 && d->q_len == d->k_len && (long long)d->map_h * d->map_w == d->q_len,
                      "attention: a position bias needs q_len == k_len == map_h * map_w (got %d, %d, %d x %d)", d->q_len, d->k_len, d->map_h,
                      d->map_w);
-        YAMD_REQUIRE(d->map_h == 1 || d->map_w <= 768, "attention: a map of several rows is at most 768 wide (got %d x %d)", d->map_h, d->map_w);
+        YAMD_REQUIRE(d->map_h == 1 || d->map_w <= 760, "attention: a map of several rows is at most 760 wide (got %d x %d)", d->map_h, d->map_w);
     }
     return YAMD_OK;
 }
@@ -378,20 +389,28 @@ FwdPlan plan_forward(const yamd_attention_desc *d, bool biased)
     return p;
 }
 
-template <int D, bool BIAS>
+template <int D, int BIAS, bool EXACT>
 int launch_forward(const AttnFwdArgs &a, long long rows, hipStream_t st)
 {
-    using Attr = KernelAttr<&attention_kernel<D, BIAS>, FwdLds<D>::most(BIAS)>;
+    using Attr = KernelAttr<&attention_kernel<D, BIAS, EXACT>, FwdLds<D>::most(BIAS)>;
     const int lds = FwdLds<D>::WINDOW + 2 * a.window * (int)sizeof(float);
     const int rc = Attr::ensure();
     if (rc != YAMD_OK) return rc;
-    hipLaunchKernelGGL((attention_kernel<D, BIAS>), dim3(work_grid(a.total)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attention_kernel<D, BIAS, EXACT>), dim3(work_grid(a.total)), dim3(256), lds, st, a);
     YAMD_LAUNCH_CHECK();
     if (a.splits > 1) {
         hipLaunchKernelGGL((attention_join_kernel<D>), dim3(ceil_div(rows, 4)), dim3(256), 0, st, a, rows);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;
+}
+
+template <int D>
+int launch_forward(Bias form, const AttnFwdArgs &a, long long rows, hipStream_t st)
+{
+    if (form == kNoBias) return launch_forward<D, kNoBias, false>(a, rows, st);
+    if (form == kQuadBias) return a.o_exact ? launch_forward<D, kQuadBias, true>(a, rows, st) : launch_forward<D, kQuadBias, false>(a, rows, st);
+    return a.o_exact ? launch_forward<D, kAnyBias, true>(a, rows, st) : launch_forward<D, kAnyBias, false>(a, rows, st);
 }
 
 }  // namespace
@@ -406,8 +425,8 @@ extern "C" size_t yamd_attention_workspace_bytes(const yamd_attention_desc *d, i
 }
 
 extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
-                              const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, float *lse,
-                              void *workspace, size_t workspace_bytes, void *stream)
+                              const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, float *o_exact,
+                              float *lse, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_attention(d, key_mask, mask_stride, bias);
     if (rc == YAMD_OK) rc = check_tokens(d, q, d->q_len, d->heads, "q");
@@ -415,6 +434,7 @@ extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q
     if (rc == YAMD_OK) rc = check_tokens(d, v, d->k_len, d->kv_heads, "v");
     if (rc == YAMD_OK) rc = check_tokens(d, o, d->q_len, d->heads, "o");
     if (rc != YAMD_OK) return rc;
+    YAMD_REQUIRE(!o_exact || (bias && ((uintptr_t)o_exact & 15) == 0), "attention: o_exact goes with a bias and is 16-byte aligned");
     const FwdPlan p = plan_forward(d, bias != nullptr);
     YAMD_REQUIRE(p.total <= (1ll << 30), "attention: %lld workgroups", p.total);
     if (p.workspace && (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15))) {
@@ -424,7 +444,7 @@ extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q
     AttnFwdArgs a = {};
     a.q = view_of(q); a.k = view_of(k); a.v = view_of(v);
     a.o = (__bf16 *)o->data; a.o_sb = o->batch_stride; a.o_st = o->token_stride; a.o_sh = o->head_stride;
-    a.lse = lse; a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
+    a.lse = lse; a.o_exact = o_exact; a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
     if (bias) {
         a.map_w = d->map_h > 1 ? d->map_w : 1;       // (of a sequence the coordinate is the position, also beyond its end)
         a.coord_last = map_coord(d->k_len - 1, a.map_w);
@@ -440,18 +460,11 @@ extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q
         a.part_ml = a.part_o + (size_t)p.splits * rows * p.dpad;
     }
     hipStream_t st = (hipStream_t)stream;
-    if (bias) {
-        switch (p.dpad) {
-        case 32: return launch_forward<32, true>(a, rows, st);
-        case 64: return launch_forward<64, true>(a, rows, st);
-        case 96: return launch_forward<96, true>(a, rows, st);
-        default: return launch_forward<128, true>(a, rows, st);
-        }
-    }
+    const Bias form = bias_form(bias, d->map_h, d->map_w);
     switch (p.dpad) {
-    case 32: return launch_forward<32, false>(a, rows, st);
-    case 64: return launch_forward<64, false>(a, rows, st);
-    case 96: return launch_forward<96, false>(a, rows, st);
-    default: return launch_forward<128, false>(a, rows, st);
+    case 32: return launch_forward<32>(form, a, rows, st);
+    case 64: return launch_forward<64>(form, a, rows, st);
+    case 96: return launch_forward<96>(form, a, rows, st);
+    default: return launch_forward<128>(form, a, rows, st);
     }
 }

@@ -11,11 +11,13 @@
 #include "yamd_attention.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace yamd {
 
 struct AttnBwdArgs {
     AttnView q, k, v, o, go;
+    const float *o_exact;          // [batch][heads][q_len][d], in the place of o where the bias has a gradient
     const float *lse;
     float *delta;                  // [batch][heads][q_len]: D
     const uint8_t *mask;
@@ -35,8 +37,12 @@ struct AttnBwdArgs {
 
 // the two rings of a wave lie 36 banks apart: the halves hold distances 4 apart, so that their 64 lanes meet 64 banks
 constexpr int kRingPad = 36;
+constexpr int kMostRing = 2048;                // positions for the widest map (w = 760: 2 * 128 + 8 + 2 * 128 + 2 w)
 
 // D = rowsum(do o): 16 lanes per row, 8 channels each.  A row without keys (lse = -inf) has no gradient whatever do holds.
+// An error e of D adds -e P to a row's dS.  For dq, dk and dv that is far below the rounding of dS; the sums of a bias bucket
+// that holds most of a row's probability, where dS cancels, feel it in full (o rounded to bf16 left the table's gradient
+// 5e-3 off), so where the bias has a gradient o comes unrounded.
 __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
 {
     const long long rows = (long long)a.batch * a.heads * a.q_len;
@@ -48,10 +54,16 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
         const int head = (int)(at % a.heads), i = (int)(at / a.heads % a.q_len);
         const long long b = at / a.heads / a.q_len;
         if (c < a.d) {
-            const bf16x8 o = *(const bf16x8 *)(a.o.p + b * a.o.sb + (long long)i * a.o.st + head * a.o.sh + c);
             const bf16x8 g = *(const bf16x8 *)(a.go.p + b * a.go.sb + (long long)i * a.go.st + head * a.go.sh + c);
+            if (a.o_exact) {
+                const f32x4 *o = (const f32x4 *)(a.o_exact + ((b * a.heads + head) * a.q_len + i) * a.d + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += (float)o[e] * (float)g[e];
+                for (int e = 0; e < 8; ++e) s += o[e >> 2][e & 3] * (float)g[e];
+            } else {
+                const bf16x8 o = *(const bf16x8 *)(a.o.p + b * a.o.sb + (long long)i * a.o.st + head * a.o.sh + c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s += (float)o[e] * (float)g[e];
+            }
         }
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) s += __shfl_xor(s, d);
@@ -74,7 +86,7 @@ struct KvLds {
     static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 : 0); }
 };
 
-template <int D, bool BIAS>
+template <int D, int BIAS>
 __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
 {
     using L = KvLds<D>;
@@ -169,10 +181,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
             lse_s[lane] = lse_n == -INFINITY ? -INFINITY : -lse_n * inv_scale;
             delta[lane] = -delta_n;
         }
-        if (BIAS && tid < ROWS) {
-            const int i = t % q_tiles * ROWS + tid;
-            coord[tid] = map_coord(i < a.q_len ? i : a.q_len - 1, a.map_w);
-        }
+        if (BIAS && tid < ROWS) coord[tid] = map_coord(t % q_tiles * ROWS + tid, a.map_w);      // (queries beyond the last one continue)
         landed();
         __syncthreads();
         // read from LDS by all waves, so that they agree on the barrier below
@@ -198,18 +207,13 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
             for (int ks = 0; ks < NKS; ++ks) gr[ks] = reader.rows(gt, 32 * u, ks);
             // both products start from a row's statistics: s from -lse / scale, dP from -D
             f32x16 s, g;
-            int at[BIAS ? 16 : 1];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[r] = lse_s[32 * u + acc_row(r, half)];
                 g[r] = delta[32 * u + acc_row(r, half)];
-                if constexpr (BIAS) at[r] = coord[32 * u + acc_row(r, half)];
             }
-            float bias_of[BIAS ? 16 : 1];
-            if constexpr (BIAS) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) bias_of[r] = win[at[r]];
-            }
+            float bias_of[16];
+            if constexpr (BIAS) read_bias<BIAS, 1>(bias_of, win, coord, u, half);
             if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) s = mfma(qr[ks], kf[ks], s);
@@ -287,14 +291,28 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
 // keys advance the distances fall: those above a(last query) - a(first key of the next tile) are final, and after each
 // tile the workgroup adds the eight rings in a fixed order for them, writes them to its row of the workspace and
 // clears them.  The ring must hold the distances of two tiles (one being added to while the other is written out):
-// 2 * 127 + 1 positions, and where a map has several rows 127 + 127 + 2 w more.
+// 2 * 127 + 1 positions and the 4 below that quads touch, and where a map has several rows 127 + 127 + 2 w more.
+// Four queries (lanes 4 i .. 4 i + 3) by four keys (accumulator rows r0 .. r0 + 3), both next to each other: lane 4 i + t
+// gets the sum of the diagonal that its own query makes with the first key (near), and of the one four distances below
+// (far; nothing for t = 0).  Half the additions to the ring are left.
+__device__ __forceinline__ void quad_diagonals(const f32x16 &g, int r0, int lane, float &near, float &far)
+{
+    const int t = lane & 3;
+    const float m1 = t < 3 ? 1.0f : 0.0f, m2 = t < 2 ? 1.0f : 0.0f, m3 = t < 1 ? 1.0f : 0.0f;
+    auto from = [&](float v, auto ctrl) {          // the value of lane (t + ctrl's rotation) % 4 of the four
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    const float x1 = from(g[r0 + 1], std::integral_constant<int, 0x39>{}), x2 = from(g[r0 + 2], std::integral_constant<int, 0x4e>{}),
+                x3 = from(g[r0 + 3], std::integral_constant<int, 0x93>{});
+    near = __builtin_fmaf(x3, m3, __builtin_fmaf(x2, m2, __builtin_fmaf(x1, m1, g[r0])));
+    far = __builtin_fmaf(x3, 1.0f - m3, __builtin_fmaf(x2, 1.0f - m2, x1 * (1.0f - m1)));
+}
+
 template <int D>
 struct QLds {
     static constexpr int T = Tile<D>::bytes(kTile), BUF = 2 * T, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
-    static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 + 8 * (2048 + kRingPad) * 4 : 0); }
-};
-
-template <int D, bool BIAS>
+    static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 + 8 * (kMostRing + kRingPad) * 4 : 0); }
+};template <int D, int BIAS>
 __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 {
     using L = QLds<D>;
@@ -411,7 +429,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         if (mp) keep &= *kept;                         // (from LDS: all waves agree on the barrier below)
         keep = uniform64(keep);
         if (t + 1 < t1) fetch(t + 1);
-        if constexpr (BIAS) flush(c_last - map_coord(t * kTile, a.map_w) + 1);   // what the tiles before this one left final
+        if (BIAS && a.part_bias) flush(c_last - map_coord(t * kTile, a.map_w) + 1);   // what the tiles before this one left final
         if (keep == 0) continue;
         if (keep != ~0ull) {                           // a masked key may hold anything, NaN included
             clear_rows<D>(kt, keep);
@@ -420,92 +438,89 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         }
         if (!busy) continue;
         const float *const win = (const float *)(smem + L::WINDOW) + (t & 1) * a.window + (BIAS ? cq - window_from(t) : 0);
-        // P and dS of 32 keys: s holds the scores, g dP
-        auto score_gradient = [&](f32x16 &s, f32x16 &g, int u) {
-            float x[BIAS ? 16 : 1];
-            if constexpr (BIAS) {
+        // The additions to the ring stand between the products, which hide part of their latency.  Narrow heads take both
+        // halves of the tile at once and make two additions at a time: keys 32 apart never put two lanes at one distance,
+        // because 32 queries are less than 32 apart.
+        constexpr int U = EARLY ? 2 : 1;
+        auto add = [&](const int (&d)[U], const float (&v)[U]) {
+            float *p[U], x[U];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(win[-coord[32 * u + acc_row(r, half)]], kLog2e, -lse2);
-            }
-            if (keep != ~0ull) mask_rows(s, keep, u, half);
+            for (int u = 0; u < U; ++u) p[u] = ring + (d[u] & (a.ring - 1));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) g[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, BIAS ? x[r] : -lse2)) * (g[r] - delta);
+            for (int u = 0; u < U; ++u) x[u] = *p[u];
+#pragma unroll
+            for (int u = 0; u < U; ++u) *p[u] = x[u] + v[u];
+            asm volatile("" ::: "memory");                   // the next addition may read what another lane wrote here
         };
-        if constexpr (EARLY) {
-            bf16x8 kr[2][NKS], vr[2][NKS];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+        for (int u0 = 0; u0 < 2; u0 += U) {
+            bf16x8 kr[U][NKS], vr[U][NKS];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int ks = 0; ks < NKS; ++ks) {
-                    kr[u][ks] = reader.rows(kt, 32 * u, ks);
-                    vr[u][ks] = reader.rows(vt, 32 * u, ks);
+                    kr[u][ks] = reader.rows(kt, 32 * (u0 + u), ks);
+                    vr[u][ks] = reader.rows(vt, 32 * (u0 + u), ks);
                 }
-            __builtin_amdgcn_sched_barrier(0);
-            f32x16 s[2], g[2];
+            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+            f32x16 s[U], g[U];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 s[u] = zero16(), g[u] = zero16();
 #pragma unroll
                 for (int ks = 0; ks < NKS; ++ks) s[u] = mfma(kr[u][ks], qf[ks], s[u]);
 #pragma unroll
                 for (int ks = 0; ks < NKS; ++ks) g[u] = mfma(vr[u][ks], gf[ks], g[u]);
             }
-            bf16x8 kx[4][NB];
+            bf16x8 kx[2 * U][NB];
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
+            for (int w = 0; w < 2 * U; ++w)
 #pragma unroll
-                for (int n = 0; n < NB; ++n) kx[w][n] = reader.transposed(kt, 16 * w, n);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int n = 0; n < NB; ++n) kx[w][n] = reader.transposed(kt, 32 * u0 + 16 * w, n);
+            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                score_gradient(s[u], g[u], u);
-                if constexpr (BIAS) __builtin_amdgcn_sched_barrier(0);
+            for (int u = 0; u < U; ++u) {                    // g: dP to dS
+                float x[16];
+                if constexpr (BIAS) {
+                    read_bias<BIAS, -1>(x, win, coord, u0 + u, half);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], kLog2e, -lse2);
+                }
+                if (keep != ~0ull) mask_rows(s[u], keep, u0 + u, half);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    g[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c2, BIAS ? x[r] : -lse2)) * (g[u][r] - delta);
+                if constexpr (EARLY && BIAS) __builtin_amdgcn_sched_barrier(0);
             }
-            asm volatile("" ::: "memory");                   // (the coordinates are read again below, not kept)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < 2 * U; ++w) {
                 const bf16x8 sf = acc_operand(g[w >> 1], w & 1);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) dq[n] = mfma(kx[w][n], sf, dq[n]);
-                if constexpr (BIAS) {
-                    // keys 32 apart are at least 32 distances apart: two additions at a time cannot meet
+                // accumulator rows that go to the ring beside this product
+                constexpr int PER = 16 / (2 * U);
 #pragma unroll
-                    for (int r = 4 * w; r < 4 * w + 4; ++r) {
-                        float *const p0 = ring + ((cq - coord[acc_row(r, half)]) & (a.ring - 1));
-                        float *const p1 = ring + ((cq - coord[32 + acc_row(r, half)]) & (a.ring - 1));
-                        const float x0 = *p0, x1 = *p1;
-                        *p0 = x0 + g[0][r];
-                        *p1 = x1 + g[1][r];
-                        asm volatile("" ::: "memory");       // the next addition may read what another lane wrote here
+                for (int r = PER * w; BIAS && r < PER * w + PER; r += BIAS == kQuadBias ? 4 : 1) {
+                    if (!a.part_bias) break;                 // a bias without gradient
+                    int d[U];
+                    float v[U], far[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        d[u] = cq - coord[32 * (u0 + u) + acc_row(r, half)];
+                        v[u] = g[u][r];
+                        if constexpr (BIAS == kQuadBias) quad_diagonals(g[u], r, lane, v[u], far[u]);
                     }
-                }
-            }
-        } else {
+                    add(d, v);
+                    if constexpr (BIAS == kQuadBias) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                f32x16 s = zero16(), g = zero16();
-#pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) s = mfma(reader.rows(kt, 32 * u, ks), qf[ks], s);
-#pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) g = mfma(reader.rows(vt, 32 * u, ks), gf[ks], g);
-                score_gradient(s, g, u);
-                if constexpr (BIAS) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        ring[(cq - coord[32 * u + acc_row(r, half)]) & (a.ring - 1)] += g[r];
-                        asm volatile("" ::: "memory");
+                        for (int u = 0; u < U; ++u) d[u] -= 4;
+                        add(d, far);
                     }
-                }
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const bf16x8 sf = acc_operand(g, w);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) dq[n] = mfma(reader.transposed(kt, 32 * u + 16 * w, n), sf, dq[n]);
                 }
             }
         }
     }
-    if constexpr (BIAS) {
+    if (BIAS && a.part_bias) {
         __syncthreads();
         flush(c_first - a.coord_last);
     }
@@ -625,7 +640,7 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     const size_t pq = p.q_splits > 1 ? (size_t)p.q_splits * bh * d->q_len * p.dpad * sizeof(float) : 0;
     p.parts = up256(pk > pq ? pk : pq);
     if (biased) {
-        const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
+        const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + 8 + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
         for (p.ring = 256; p.ring < span; p.ring *= 2) {}
         const int coord_last = map_coord(d->k_len - 1, w);
         p.part_len = coord_last + kBlockRows + (d->map_h > 1 ? kBlockRows + w : 0);
@@ -635,7 +650,7 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     return p;
 }
 
-template <int D, bool BIAS>
+template <int D, int BIAS>
 int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv, float *dbias,
                     hipStream_t st)
 {
@@ -672,11 +687,20 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
         rc = launch_sum_parts(w, w.part0, a.heads, a.q_len, D, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh, st);
         if (rc != YAMD_OK) return rc;
     }
-    if (BIAS) {
+    if (BIAS && dbias) {
         hipLaunchKernelGGL(attention_bias_grad_kernel, dim3(ceil_div(a.n_off, 64), a.heads), dim3(1024), 0, st, w, dbias);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;
+}
+
+template <int D>
+int launch_backward(Bias form, const AttnBwdArgs &a, const BwdPlan &p, const yamd_tokens *dq, const yamd_tokens *dk, const yamd_tokens *dv,
+                    float *dbias, hipStream_t st)
+{
+    if (form == kQuadBias) return launch_backward<D, kQuadBias>(a, p, dq, dk, dv, dbias, st);
+    return form == kAnyBias ? launch_backward<D, kAnyBias>(a, p, dq, dk, dv, dbias, st)
+                            : launch_backward<D, kNoBias>(a, p, dq, dk, dv, dbias, st);
 }
 
 }  // namespace
@@ -693,7 +717,7 @@ extern "C" size_t yamd_attention_backward_workspace_bytes(const yamd_attention_d
 
 extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
                                        const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,
-                                       const float *lse, const yamd_tokens *d_o, const yamd_tokens *dq, const yamd_tokens *dk,
+                                       const float *o_exact, const float *lse, const yamd_tokens *d_o, const yamd_tokens *dq, const yamd_tokens *dk,
                                        const yamd_tokens *dv, float *dbias, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_attention(d, key_mask, mask_stride, bias);
@@ -707,7 +731,8 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     if (rc == YAMD_OK) rc = check_tokens(d, dv, d->k_len, d->kv_heads, "dv");
     if (rc != YAMD_OK) return rc;
     YAMD_REQUIRE(lse, "attention backward: lse is null");
-    YAMD_REQUIRE((bias == nullptr) == (dbias == nullptr), "attention backward: bias and its gradient go together");
+    YAMD_REQUIRE(!dbias || bias, "attention backward: a bias gradient without a bias");
+    YAMD_REQUIRE(!dbias || (o_exact && ((uintptr_t)o_exact & 15) == 0), "attention backward: a bias gradient needs o_exact (16-byte aligned)");
     const BwdPlan p = plan_backward(d, bias != nullptr);
     YAMD_REQUIRE(p.kv_total <= (1ll << 30) && p.q_total <= (1ll << 30), "attention backward: too many workgroups");
     if (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15)) {
@@ -719,7 +744,8 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     a.lse = lse;
     a.delta = (float *)workspace;
     a.part0 = (float *)((char *)workspace + p.delta);
-    a.part_bias = (float *)((char *)workspace + p.delta + p.parts);
+    a.part_bias = dbias ? (float *)((char *)workspace + p.delta + p.parts) : nullptr;
+    a.o_exact = dbias ? o_exact : nullptr;
     a.ring = p.ring;
     a.part_len = p.part_len;
     a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
@@ -732,18 +758,11 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     a.batch = d->batch; a.q_len = d->q_len; a.k_len = d->k_len; a.d = d->head_dim;
     a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads; a.scale = d->scale;
     hipStream_t st = (hipStream_t)stream;
-    if (bias) {
-        switch (p.dpad) {
-        case 32: return launch_backward<32, true>(a, p, dq, dk, dv, dbias, st);
-        case 64: return launch_backward<64, true>(a, p, dq, dk, dv, dbias, st);
-        case 96: return launch_backward<96, true>(a, p, dq, dk, dv, dbias, st);
-        default: return launch_backward<128, true>(a, p, dq, dk, dv, dbias, st);
-        }
-    }
+    const Bias form = bias_form(bias, d->map_h, d->map_w);
     switch (p.dpad) {
-    case 32: return launch_backward<32, false>(a, p, dq, dk, dv, dbias, st);
-    case 64: return launch_backward<64, false>(a, p, dq, dk, dv, dbias, st);
-    case 96: return launch_backward<96, false>(a, p, dq, dk, dv, dbias, st);
-    default: return launch_backward<128, false>(a, p, dq, dk, dv, dbias, st);
+    case 32: return launch_backward<32>(form, a, p, dq, dk, dv, dbias, st);
+    case 64: return launch_backward<64>(form, a, p, dq, dk, dv, dbias, st);
+    case 96: return launch_backward<96>(form, a, p, dq, dk, dv, dbias, st);
+    default: return launch_backward<128>(form, a, p, dq, dk, dv, dbias, st);
     }
 }

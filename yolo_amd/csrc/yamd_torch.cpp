@@ -239,7 +239,7 @@ yamd_attention_desc descriptor(const Tensor &q, const Tensor &k, double scale, i
 }
 
 struct AttentionOut {
-    Tensor o, lse;
+    Tensor o, lse, exact;
 };
 
 AttentionOut attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &mask, const Tensor &bias, double scale, int64_t h,
@@ -258,13 +258,15 @@ AttentionOut attention_forward(const Tensor &q, const Tensor &k, const Tensor &v
         return r;
     }
     r.o = at::empty(q.sizes(), q.options());
+    if (stats && bias.defined() && bias.requires_grad())
+        r.exact = at::empty({q.size(0), q.size(2), q.size(1), q.size(3)}, q.options().dtype(at::kFloat));
     const yamd_attention_desc d = descriptor(q, k, scale, h, w);
     const yamd_tokens tq = tokens(q), tk = tokens(k), tv = tokens(v), to = tokens(r.o);
     const size_t nbytes = yamd_attention_workspace_bytes(&d, bias.defined());
     Tensor ws;
     if (nbytes) ws = bytes(nbytes, q);
     check(yamd_attention(&d, &tq, &tk, &tv, (const uint8_t *)ptr(mask), mask.defined() ? mask.stride(0) : 0, (const float *)ptr(bias), &to,
-                         (float *)ptr(r.lse), ptr(ws), nbytes, stream_of(q)),
+                         (float *)ptr(r.exact), (float *)ptr(r.lse), ptr(ws), nbytes, stream_of(q)),
           "attention");
     return r;
 }
@@ -275,7 +277,7 @@ struct Attention : Function<Attention> {
     {
         const Tensor bias = bias_.value_or(Tensor()), mask = mask_.value_or(Tensor());
         AttentionOut r = attention_forward(q, k, v, mask, bias, scale, h, w, true);
-        ctx->save_for_backward({q, k, v, bias, mask, r.o, r.lse});
+        ctx->save_for_backward({q, k, v, bias, mask, r.o, r.lse, r.exact});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["h"] = h;
         ctx->saved_data["w"] = w;
@@ -285,12 +287,12 @@ struct Attention : Function<Attention> {
     {
         once_only("attention");
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &v = s[2], &bias = s[3], &mask = s[4], &o = s[5], &lse = s[6];
+        const Tensor &q = s[0], &k = s[1], &v = s[2], &bias = s[3], &mask = s[4], &o = s[5], &lse = s[6], &exact = s[7];
         const c10::DeviceGuard guard(q.device());
         const bool nothing = q.numel() == 0 || k.numel() == 0;
         auto result = [&](const Tensor &t) { return nothing ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options()); };
         Tensor dq = result(q), dk = result(k), dv = result(v), dbias;
-        if (bias.defined()) dbias = result(bias);
+        if (bias.defined() && ctx->needs_input_grad(3)) dbias = result(bias);
         if (!nothing) {
             const Tensor go = grads[0].contiguous();
             const yamd_attention_desc d = descriptor(q, k, ctx->saved_data["scale"].toDouble(), ctx->saved_data["h"].toInt(),
@@ -300,7 +302,8 @@ struct Attention : Function<Attention> {
             const size_t nbytes = yamd_attention_backward_workspace_bytes(&d, bias.defined());
             const Tensor ws = bytes(nbytes, q);
             check(yamd_attention_backward(&d, &tq, &tk, &tv, (const uint8_t *)ptr(mask), mask.defined() ? mask.stride(0) : 0,
-                                          (const float *)ptr(bias), &to, (const float *)lse.data_ptr(), &tg, &tdq, &tdk, &tdv,
+                                          (const float *)ptr(bias), &to, (const float *)ptr(exact),
+                                          (const float *)lse.data_ptr(), &tg, &tdq, &tdk, &tdv,
                                           (float *)ptr(dbias), ws.data_ptr(), nbytes, stream_of(q)),
                   "attention_backward");
         }

@@ -154,10 +154,11 @@ def _load() -> ctypes.CDLL:
     T = P(Tokens)
     lib.yamd_attention_workspace_bytes.restype = c_size_t
     lib.yamd_attention_workspace_bytes.argtypes = [P(AttentionDesc), c_int]
-    lib.yamd_attention.argtypes = [P(AttentionDesc), T, T, T, c_void_p, c_longlong, c_void_p, T, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.yamd_attention.argtypes = [P(AttentionDesc), T, T, T, c_void_p, c_longlong, c_void_p, T, c_void_p, c_void_p, c_void_p, c_size_t,
+                                   c_void_p]
     lib.yamd_attention_backward_workspace_bytes.restype = c_size_t
     lib.yamd_attention_backward_workspace_bytes.argtypes = [P(AttentionDesc), c_int]
-    lib.yamd_attention_backward.argtypes = [P(AttentionDesc), T, T, T, c_void_p, c_longlong, c_void_p, T, c_void_p, T, T, T, T, c_void_p,
+    lib.yamd_attention_backward.argtypes = [P(AttentionDesc), T, T, T, c_void_p, c_longlong, c_void_p, T, c_void_p, c_void_p, T, T, T, T, c_void_p,
                                             c_void_p, c_size_t, c_void_p]
     lib.yamd_relative_bias.argtypes = [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]
     lib.yamd_relative_bias_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p]

@@ -59,8 +59,8 @@ class RelativePosition:
     def __init__(self, h: int, w: int, buckets: int, max_distance: int, device="cuda"):
         if h < 1 or w < 1 or h * w > 1 << 24:
             raise _lib.YamdError(f"bad map {h} x {w}")
-        if h > 1 and w > 768:
-            raise _lib.YamdError(f"a map of several rows is at most 768 wide, got {h} x {w}")
+        if h > 1 and w > 760:
+            raise _lib.YamdError(f"a map of several rows is at most 760 wide, got {h} x {w}")
         self.h, self.w, self.buckets, self.max_distance = int(h), int(w), int(buckets), int(max_distance)
         of = torch.tensor(axis_buckets(w, buckets, max_distance), dtype=torch.int64)
         self.rows = buckets
