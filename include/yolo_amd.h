@@ -408,7 +408,8 @@ typedef struct yamd_attention_desc {
  *   key_mask  (batch rows of k_len bytes, mask_stride apart; NULL = all): keys with 0 are not attended, and what k and v hold
  *             there does not matter.  A query that is left without keys gets zeros.
  *   bias      (heads rows of (2 map_h - 1)(2 map_w - 1) floats; NULL = none): added to the score of a query at (y, x) and a
- *             key at (y', x') from [(y - y' + map_h - 1)(2 map_w - 1) + x - x' + map_w - 1].
+ *             key at (y', x') from [(y - y' + map_h - 1)(2 map_w - 1) + x - x' + map_w - 1].  Biases below -1e5 (-inf, the
+ *             type's lowest value, ...) mask: a query with only such scores counts as left without keys.
  *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted; only with a bias): o before its
  *             rounding to bf16 and with probabilities kept to 16 bits, which the gradient of a bias needs.
  *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
@@ -463,13 +464,19 @@ enum {
     YAMD_OP_CONV_CAT2 = 13,       /* yamd_conv2d_bias_act_cat2: desc; p[0] = xa, p[3] = xb, p[5] = y2 or NULL;
                                    * i = {xa_cstride, xb_cstride, y_cstride, h, w, y2_cstride, split_cout, ca, xa_half | xb_half << 1} */
     YAMD_OP_BOTTLENECK = 14,      /* yamd_bottleneck: i = {x_cstride, cin, y_cstride, h, w, cmid, cout, act, shortcut} */
-    YAMD_OP_C3 = 15               /* yamd_c3_fused: i = {x_cstride, cin, y_cstride, h, w, ch, cout, act, shortcut} */
+    YAMD_OP_C3 = 15,              /* yamd_c3_fused: i = {x_cstride, cin, y_cstride, h, w, ch, cout, act, shortcut} */
+    YAMD_OP_LAYER_NORM = 16,      /* yamd_layer_norm over the channels of batch*h*w bf16 pixels, float32 p[1] = weight, p[2] = bias (or NULL),
+                                   * desc.residual_scale = eps; i = {x_cstride, y_cstride, h, w, c} */
+    YAMD_OP_ATTENTION = 17        /* yamd_attention between the pixels of two maps (channels = heads side by side): p[0] = q, p[1] = k,
+                                   * p[2] = v, p[3] = bias or NULL, p[5] = workspace, p[6] = its size in bytes (an integer);
+                                   * desc.cin = head_dim, desc.residual_scale = scale;
+                                   * i = {q_cstride, k_cstride, v_cstride, y_cstride, q_h, q_w, k_h * k_w, heads, kv_heads} */
 };
 typedef struct yamd_plan_op {
     int32_t kind;
     int32_t i[9];
     void *p[7];
-    yamd_conv_desc desc;          /* YAMD_OP_CONV / YAMD_OP_CONV_SPLIT only */
+    yamd_conv_desc desc;          /* YAMD_OP_CONV / YAMD_OP_CONV_SPLIT; single fields of it where a kind says so */
 } yamd_plan_op;
 typedef struct yamd_plan yamd_plan;
 int yamd_plan_create(const yamd_plan_op *ops, int n_ops, int batch, int img_h, int img_w, yamd_plan **plan_out);

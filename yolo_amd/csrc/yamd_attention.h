@@ -16,6 +16,7 @@ namespace yamd {
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMasked = -1e5f;         // a query whose scores with their bias are all below this is left without keys
 constexpr int kTile = 64;                // rows of a tile that passes through LDS (keys, or queries in the dK / dV kernel)
 constexpr int kBlockRows = 128;          // rows that a workgroup owns: 32 for each of its four waves
 

@@ -185,6 +185,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         top = with_other_half(top, [](float x, float y) { return fmaxf(x, y); });
         const float unit = BIAS ? kLog2e : c2;           // scores to units of log 2
         top *= unit;
+        // a tile of masking biases only: no maximum yet (differences of such numbers would mean nothing)
+        if (BIAS && top < kMasked * kLog2e) top = -INFINITY;
         if (__any(top > m)) {
             const float m_new = fmaxf(m, top);
             const float f = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));

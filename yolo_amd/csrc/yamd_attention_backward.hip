@@ -196,7 +196,8 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
                                  (BIAS ? c_key - c_low - map_coord(t % q_tiles * ROWS, a.map_w) : 0);
         if (!busy) continue;
         // Operands are requested one stage ahead of the products that use them, as far as registers allow; fences keep the
-        // scheduler from putting each read right before its product.  Columns (keys) do not mix, so a masked key's column
+        // scheduler from putting each read right before its product.  A wave has priority while it issues products, so that the
+        // other wave of its SIMD is pushed towards its arithmetic (3 % of the backward pass at d = 64).  Columns (keys) do not mix, so a masked key's column
         // may hold anything until its result is replaced by zeros at the end.
 #pragma unroll
         for (int u = 0; u < ROWS / 32; ++u) {
@@ -215,6 +216,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
             float bias_of[16];
             if constexpr (BIAS) read_bias<BIAS, 1>(bias_of, win, coord, u, half);
             if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) s = mfma(qr[ks], kf[ks], s);
 #pragma unroll
@@ -222,6 +224,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
                 if constexpr (L::VALUES) g = mfma(gr[ks], reader.rows(smem + L::V, 32 * wave, ks), g);
                 else g = mfma(gr[ks], vf[ks], g);
             }
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(0);
             bf16x8 gx[2][NB], qx[2][NB];
 #pragma unroll
             for (int w = 0; w < 2; ++w)
@@ -236,6 +239,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
                 s[r] = __builtin_amdgcn_exp2f(BIAS ? __builtin_fmaf(s[r], c2, bias_of[r] * kLog2e) : s[r] * c2);
                 g[r] *= s[r];
             }
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const bf16x8 pf = acc_operand(s, w), sf = acc_operand(g, w);
@@ -245,6 +249,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
                     dk[n] = mfma(qx[w][n], sf, dk[n]);
                 }
             }
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(0);
         }
     }
     if (key0 + c32 >= a.k_len) return;
@@ -463,6 +468,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
                     vr[u][ks] = reader.rows(vt, 32 * (u0 + u), ks);
                 }
             if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(1);
             f32x16 s[U], g[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -472,6 +478,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 #pragma unroll
                 for (int ks = 0; ks < NKS; ++ks) g[u] = mfma(vr[u][ks], gf[ks], g[u]);
             }
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(0);
             bf16x8 kx[2 * U][NB];
 #pragma unroll
             for (int w = 0; w < 2 * U; ++w)
@@ -492,6 +499,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
                     g[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c2, BIAS ? x[r] : -lse2)) * (g[u][r] - delta);
                 if constexpr (EARLY && BIAS) __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int w = 0; w < 2 * U; ++w) {
                 const bf16x8 sf = acc_operand(g[w >> 1], w & 1);
@@ -518,6 +526,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
                     }
                 }
             }
+            if constexpr (EARLY) __builtin_amdgcn_s_setprio(0);
         }
     }
     if (BIAS && a.part_bias) {

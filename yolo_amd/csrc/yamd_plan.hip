@@ -55,6 +55,25 @@ int run_op(const yamd_plan &pl, const yamd_plan_op &o, const float *images, void
         return yamd_depth_to_space2(p[0], i[0], p[4], i[1], pl.batch, i[2], i[3], i[4], st);
     case YAMD_OP_COPY_CHANNELS:
         return yamd_copy_channels(p[0], i[0], p[4], i[1], (long long)pl.batch * i[2] * i[3], i[4], st);
+    case YAMD_OP_LAYER_NORM:
+        return yamd_layer_norm(p[0], i[0], p[1], p[2], YAMD_F32, o.desc.residual_scale, p[4], i[1], nullptr, nullptr,
+                               (long long)pl.batch * i[2] * i[3], i[4], YAMD_BF16, st);
+    case YAMD_OP_ATTENTION: {
+        yamd_attention_desc d;
+        d.batch = pl.batch;
+        d.heads = i[7];
+        d.kv_heads = i[8];
+        d.head_dim = o.desc.cin;
+        d.q_len = i[4] * i[5];
+        d.k_len = i[6];
+        d.map_h = i[4];
+        d.map_w = i[5];
+        d.scale = o.desc.residual_scale;
+        auto tokens = [&](void *data, int cstride, int len) { return yamd_tokens{data, (long long)len * cstride, cstride, d.head_dim}; };
+        const yamd_tokens q = tokens(p[0], i[0], d.q_len), k = tokens(p[1], i[1], d.k_len), v = tokens(p[2], i[2], d.k_len),
+                          y = tokens(p[4], i[3], d.q_len);
+        return yamd_attention(&d, &q, &k, &v, nullptr, 0, (const float *)p[3], &y, nullptr, nullptr, p[5], (size_t)p[6], st);
+    }
     default:
         break;
     }
@@ -69,7 +88,7 @@ extern "C" int yamd_plan_create(const yamd_plan_op *ops, int n_ops, int batch, i
     YAMD_REQUIRE(ops && plan_out && n_ops > 0 && n_ops <= 65536, "bad argument (n_ops=%d)", n_ops);
     YAMD_REQUIRE(batch > 0 && img_h > 0 && img_w > 0, "bad shape %dx%dx%d", batch, img_h, img_w);
     for (int k = 0; k < n_ops; ++k)
-        YAMD_REQUIRE(ops[k].kind >= YAMD_OP_CONV && ops[k].kind <= YAMD_OP_C3, "op %d: unknown kind %d", k, ops[k].kind);
+        YAMD_REQUIRE(ops[k].kind >= YAMD_OP_CONV && ops[k].kind <= YAMD_OP_ATTENTION, "op %d: unknown kind %d", k, ops[k].kind);
     yamd_plan *pl = new (std::nothrow) yamd_plan;
     YAMD_REQUIRE(pl != nullptr, "out of host memory");
     pl->ops.assign(ops, ops + n_ops);

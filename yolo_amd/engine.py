@@ -253,6 +253,53 @@ class C3Layer:
             self.b_dev = self.b_host.to(device)
 
 
+class NormLayer:
+    """Layer norm over the channels of every pixel (``yamd_layer_norm``)."""
+
+    def __init__(self, name: str, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float):
+        host = lambda t: None if t is None else t.detach().to(torch.float32).cpu().contiguous()
+        self.name, self.eps = name, float(eps)
+        self.w_host, self.b_host = host(weight), host(bias)
+        self.w_dev: Optional[torch.Tensor] = None
+        self.b_dev: Optional[torch.Tensor] = None
+        self.device: Optional[torch.device] = None
+
+    def to(self, device) -> None:
+        if self.device != torch.device(device):
+            self.device = torch.device(device)
+            self.w_dev = None if self.w_host is None else self.w_host.to(device)
+            self.b_dev = None if self.b_host is None else self.b_host.to(device)
+
+
+class AttentionLayer:
+    """Attention between the pixels of two maps, heads side by side in the channels (``yamd_attention``); with a learned
+    position bias ``table`` / ``position`` (see ``yolo_amd.tokens``), which is expanded once per device."""
+
+    def __init__(self, name: str, heads: int, kv_heads: int, head_dim: int, q_hw: Tuple[int, int], k_len: int, scale: float,
+                 table: Optional[torch.Tensor], position):
+        self.name, self.heads, self.kv_heads, self.head_dim = name, heads, kv_heads, head_dim
+        self.q_hw, self.k_len, self.scale = q_hw, k_len, scale
+        self.table = None if table is None else table.detach().to(torch.float32).cpu().contiguous()
+        self.bucket_of = None if position is None else position.bucket_of.cpu()
+        self.w_dev: Optional[torch.Tensor] = None       # the bias by distance, on the device
+        self.b_dev = None
+        self.workspace = ""                              # its name among the program's buffers
+        self.device: Optional[torch.device] = None
+
+    def to(self, device) -> None:
+        if self.device != torch.device(device):
+            self.device = torch.device(device)
+            # (the expansion is a gather: exact wherever it runs)
+            self.w_dev = None if self.table is None else self.table[self.bucket_of.long()].t().contiguous().to(device)
+
+    def desc(self, batch: int) -> "_lib.AttentionDesc":
+        return _lib.AttentionDesc(batch, self.heads, self.kv_heads, self.head_dim, self.q_hw[0] * self.q_hw[1], self.k_len,
+                                  self.q_hw[0], self.q_hw[1], self.scale)
+
+    def workspace_bytes(self, batch: int) -> int:
+        return LIB.yamd_attention_workspace_bytes(ctypes.byref(self.desc(batch)), int(self.table is not None))
+
+
 class Program:
     def __init__(self, img_h: int, img_w: int):
         self.img_h, self.img_w = img_h, img_w
@@ -390,6 +437,44 @@ class Program:
             out = self.buffer(2 * x.h, 2 * x.w, cout)
         assert (out.h, out.w, out.c) == (2 * x.h, 2 * x.w, cout)
         self.ops.append(("d2s", t, out))
+        return out
+
+    def layer_norm(self, name: str, x: View, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5,
+                   out: Optional[View] = None) -> View:
+        """nn.LayerNorm over the channels of every pixel."""
+        for t in (weight, bias):
+            assert t is None or tuple(t.shape) == (x.c,), (name, x, t.shape)
+        if out is None:
+            out = self.buffer(x.h, x.w, x.c)
+        assert (out.h, out.w, out.c) == (x.h, x.w, x.c), (name, out, x)
+        layer = NormLayer(name, weight, bias, eps)
+        self.stems.append(layer)                            # (uploaded with the other layers)
+        self.ops.append(("norm", layer, x, out))
+        return out
+
+    def attention(self, name: str, q: View, k: View, v: View, heads: int, kv_heads: Optional[int] = None, scale: Optional[float] = None,
+                  table: Optional[torch.Tensor] = None, position=None, out: Optional[View] = None) -> View:
+        """softmax(scale * q k^T + bias) v between the pixels of q's map and those of k's and v's, ``heads`` side by side in the
+        channels (typically slices of one 1x1 conv's output).  ``table`` / ``position`` (``tokens.RelativePosition``): a
+        learned position bias, for self-attention over one map."""
+        kv_heads = heads if kv_heads is None else kv_heads
+        d = q.c // heads
+        if q.c != heads * d or k.c != kv_heads * d or v.c != k.c or (k.h, k.w) != (v.h, v.w) or heads % kv_heads:
+            raise _lib.YamdError(f"attention[{name}]: {heads} heads over {q.c} channels do not fit {kv_heads} over {k.c} and {v.c}")
+        if not 8 <= d <= 128 or d % 8 or any(t.coff % 8 or self.buffers[t.buf][2] % 8 or self.buffers[t.buf][3] != torch.bfloat16 for t in (q, k, v)):
+            raise _lib.YamdError(f"attention[{name}]: heads must be 8 to 128 channels, a multiple of 8, of bf16 maps (got {d})")
+        if (table is None) != (position is None):
+            raise _lib.YamdError(f"attention[{name}]: table and position go together")
+        if position is not None and ((position.h, position.w) != (q.h, q.w) or (k.h, k.w) != (q.h, q.w)
+                                     or tuple(table.shape) != (position.rows, heads)):
+            raise _lib.YamdError(f"attention[{name}]: a position bias needs one {q.h} x {q.w} map and a ({position.rows}, {heads}) table")
+        if out is None:
+            out = self.buffer(q.h, q.w, q.c)
+        assert (out.h, out.w, out.c) == (q.h, q.w, q.c), (name, out, q)
+        layer = AttentionLayer(name, heads, kv_heads, d, (q.h, q.w), k.h * k.w, 1.0 / d ** 0.5 if scale is None else float(scale), table, position)
+        layer.workspace = f"workspace {len(self.ops)} of {name}"
+        self.stems.append(layer)
+        self.ops.append(("attn", layer, q, k, v, out))
         return out
 
     def cat(self, views: List[View], name: Optional[str] = None) -> View:
@@ -642,6 +727,12 @@ class Program:
             return 0.0, float(batch * op[1].h * op[1].w * op[1].c * 2 * 1.25)
         if kind == "d2s":
             return 0.0, float(batch * op[1].h * op[1].w * op[1].c * 2 * 2)
+        if kind == "norm":
+            return 0.0, float(batch * op[2].h * op[2].w * op[2].c * 2 * 2)
+        if kind == "attn":
+            _, layer, q, k, v, out = op
+            byts = batch * 2 * (2 * q.h * q.w * q.c + 2 * layer.k_len * k.c)
+            return 4.0 * batch * q.h * q.w * layer.k_len * q.c, float(byts)
         return 0.0, 0.0
 
     # ---- execution -------------------------------------------------------------------------------
@@ -656,6 +747,10 @@ class Program:
             return [op[2]]
         if kind in ("up2", "copy", "d2s", "mp2", "mp5"):
             return [op[1]]
+        if kind == "norm":
+            return [op[2]]
+        if kind == "attn":
+            return list(op[2:5])
         return []
 
     def fuse_upsample_cat(self) -> int:
@@ -818,6 +913,9 @@ class Program:
             self._cplan.clear()
             self._alloc[key] = {n: torch.empty((batch, h, w, c), dtype=dt, device=device)
                                 for n, (h, w, c, dt) in self.buffers.items() if n not in self.alias}
+            for op in self.ops:
+                if op[0] == "attn" and op[1].workspace_bytes(batch):
+                    self._alloc[key][op[1].workspace] = torch.empty(op[1].workspace_bytes(batch), dtype=torch.uint8, device=device)
             for layer in self.convs + self.stems:
                 layer.to(device)
         return self._alloc[key]
@@ -924,9 +1022,27 @@ class Program:
                         "mp2": _lib.OP_MAXPOOL2}[kind]
                 fill(code, (xcs, ycs, x.h, x.w, out.c if kind == "d2s" else x.c), {0: xp, 4: yp})
                 names.append(kind)
+            elif kind == "norm":
+                _, layer, x, out = op
+                xp, xcs = P(bufs, x)
+                yp, ycs = P(bufs, out)
+                o.desc.residual_scale = layer.eps
+                fill(_lib.OP_LAYER_NORM, (xcs, ycs, x.h, x.w, x.c),
+                     {0: xp, 1: None if layer.w_dev is None else layer.w_dev.data_ptr(),
+                      2: None if layer.b_dev is None else layer.b_dev.data_ptr(), 4: yp})
+                names.append(f"layer_norm[{layer.name}]")
+            elif kind == "attn":
+                _, layer, q, k, v, out = op
+                ptrs = [P(bufs, t) for t in (q, k, v, out)]
+                ws = bufs.get(layer.workspace)
+                o.desc.cin, o.desc.residual_scale = layer.head_dim, layer.scale
+                fill(_lib.OP_ATTENTION, (*(cs for _, cs in ptrs), q.h, q.w, layer.k_len, layer.heads, layer.kv_heads),
+                     {0: ptrs[0][0], 1: ptrs[1][0], 2: ptrs[2][0], 3: None if layer.w_dev is None else layer.w_dev.data_ptr(), 4: ptrs[3][0],
+                      5: None if ws is None else ws.data_ptr(), 6: 0 if ws is None else ws.numel()})
+                names.append(f"attention[{layer.name}]")
             else:
                 raise AssertionError(kind)
-        keep = tuple(bufs.values()) + tuple(t for layer in self.convs + self.stems for t in (layer.w_dev, layer.b_dev))
+        keep = tuple(bufs.values()) + tuple(t for layer in self.convs + self.stems for t in (layer.w_dev, layer.b_dev) if t is not None)
         plan = _CPlan(ops, batch, self.img_h, self.img_w, names, keep)
         self._cplan[key] = plan
         return plan
@@ -1052,6 +1168,22 @@ class Program:
                 xp, xcs = P(bufs, x)
                 yp, ycs = P(bufs, out)
                 _lib.check(LIB.yamd_maxpool2(xp, xcs, yp, ycs, B, x.h, x.w, x.c, st), "maxpool2")
+            elif kind == "norm":
+                _, layer, x, out = op
+                xp, xcs = P(bufs, x)
+                yp, ycs = P(bufs, out)
+                _lib.check(LIB.yamd_layer_norm(xp, xcs, None if layer.w_dev is None else layer.w_dev.data_ptr(),
+                                               None if layer.b_dev is None else layer.b_dev.data_ptr(), _lib.DTYPE_F32, layer.eps, yp, ycs,
+                                               None, None, B * x.h * x.w, x.c, _lib.DTYPE_BF16, st), f"layer_norm[{layer.name}]")
+            elif kind == "attn":
+                _, layer, q, k, v, out = op
+                toks = [_lib.Tokens(ptr, t.h * t.w * cs, cs, layer.head_dim) for t in (q, k, v, out) for ptr, cs in (P(bufs, t),)]
+                ws = bufs.get(layer.workspace)
+                d = layer.desc(B)
+                _lib.check(LIB.yamd_attention(ctypes.byref(d), *(ctypes.byref(t) for t in toks[:3]), None, 0,
+                                              None if layer.w_dev is None else layer.w_dev.data_ptr(), ctypes.byref(toks[3]), None, None,
+                                              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), st),
+                           f"attention[{layer.name}]")
             else:
                 raise AssertionError(kind)
             if timings is not None:
@@ -1060,7 +1192,7 @@ class Program:
                 if kind in ("stem", "stem2", "conv_cat2", "bneck", "c3"):          # reported with the convs
                     timings.append(("conv", op[1].name, ev0, ev1) + self.op_cost(op, B))
                 else:
-                    timings.append((kind, op[1].name if kind == "conv" else kind, ev0, ev1) + self.op_cost(op, B))
+                    timings.append((kind, op[1].name if kind in ("conv", "norm", "attn") else kind, ev0, ev1) + self.op_cost(op, B))
         if span_open is not None:
             ev = torch.cuda.Event(enable_timing=True)
             ev.record()

@@ -33,7 +33,8 @@ EXPORTS = [
 
 # yamd_plan_op.kind
 OP_CONV, OP_CONV_SPLIT, OP_STEM, OP_STEM_CONV2, OP_FOCUS, OP_NHWC16, OP_UPSAMPLE2X, OP_MAXPOOL5_CASCADE, \
-    OP_MAXPOOL3_CASCADE, OP_MAXPOOL2, OP_DEPTH_TO_SPACE2, OP_COPY_CHANNELS, OP_CONV_CAT2, OP_BOTTLENECK, OP_C3 = range(1, 16)
+    OP_MAXPOOL3_CASCADE, OP_MAXPOOL2, OP_DEPTH_TO_SPACE2, OP_COPY_CHANNELS, OP_CONV_CAT2, OP_BOTTLENECK, OP_C3, \
+    OP_LAYER_NORM, OP_ATTENTION = range(1, 18)
 
 
 class ConvDesc(ctypes.Structure):
