@@ -266,8 +266,9 @@ int check_attention(const yamd_attention_desc *d, const uint8_t *key_mask, long 
 int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, int heads, const char *name);
 static inline AttnView view_of(const yamd_tokens *t) { return {(const __bf16 *)t->data, t->batch_stride, t->token_stride, t->head_stride}; }
 
-// split of the looped axis when the owned rows alone give too few workgroups: the number of parts of `tiles` tiles
-int attention_splits(long long workgroups, int tiles, int min_tiles);
+// split of the looped axis when the owned rows alone give too few workgroups: the number of parts of `tiles` tiles, for
+// `rows` rows of results, with `resident` workgroups on a CU at a time (what their registers allow)
+int attention_splits(long long workgroups, int tiles, long long rows, int resident);
 
 // head width of the kernel that serves `d` channels: the channels beyond d are zeros in registers and LDS
 static inline int padded_head_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }

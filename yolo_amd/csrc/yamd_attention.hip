@@ -108,9 +108,9 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         clear_lds(smem, 2 * L::BUF);
         __syncthreads();
     }
+    if (t0 < t1) fetch(t0);
     // (a wait that the compiler sees: it would otherwise wait for the query rows inside the loop, and for the tiles with them)
     __builtin_amdgcn_s_waitcnt(0x0f70);
-    if (t0 < t1) fetch(t0);
     TileReader<D> reader(lane);
     for (int t = t0; t < t1; ++t) {
         if constexpr (D > 64) reader.forget();
@@ -265,14 +265,18 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
         a.lse[((long long)b * a.heads + head) * a.q_len + i] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
-// Joins the parts of a split key axis: one wave per row.  A lane owns 4 channels, and the 64 / (D / 4) groups of lanes take
-// the parts in turns, four at a time so that their loads overlap; the groups are joined by exchanges in a fixed order.
+// Joins the parts of a split key axis.  A lane owns 4 channels of a row and takes its parts four at a time, so that their
+// loads overlap.  With many parts a wave works on one row: its 64 / (D / 4) groups of lanes take the parts in turns and are
+// joined by exchanges in a fixed order (33 parts of 2400 rows, D 32: 4 us against 18 without); with up to 8 parts the groups
+// take a row each (3 parts of 26046 rows, D 64: 7 us against 14).
 template <int D>
+constexpr int kJoinLanes = D == 96 ? 32 : D / 4;               // (of 32 lanes 24 work for D = 96)
+template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long long rows)
 {
-    constexpr int CH = D == 96 ? 32 : D / 4, G = 64 / CH;      // (of 32 lanes 24 work for D = 96)
-    const int lane = threadIdx.x & 63, g = lane / CH, c = 4 * (lane % CH);
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int CH = kJoinLanes<D>, G = SHARED ? 64 / CH : 1;
+    const int lane = threadIdx.x & 63, g = SHARED ? lane / CH : 0, c = 4 * (lane % CH);
+    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / (CH * G);
     if (at >= rows) return;
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long
         for (int k = 0; k < 4; ++k) merge(ml[k].x, ml[k].y, po[k]);
     }
 #pragma unroll
-    for (int d = CH; d < 64; d <<= 1) {
+    for (int d = CH; SHARED && d < 64; d <<= 1) {
         const float pm = __shfl_xor(m, d), pl = __shfl_xor(l, d);
         f32x4 po;
 #pragma unroll
@@ -319,7 +323,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long
         if (a.o_exact) *(f32x4 *)(a.o_exact + at * a.d + c) = o;
         *(bf16x4 *)(a.o + bh / a.heads * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
     }
-    if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
+    if (a.lse && g == 0 && c == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
@@ -355,12 +359,29 @@ int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
     return YAMD_OK;
 }
 
-int attention_splits(long long workgroups, int tiles, int min_tiles)
+// Parts that the looped axis of `tiles` tiles is split into.  From 512 workgroups on there is nothing to gain (800 workgroups
+// of 100 tiles, d 64: 276 us whole, 284 in two parts; 832 of 25: 97 and 125).  Below, the cost in units of a tile's time
+// is that of a CU with n workgroups, `resident` at a time and each `steps` tiles long (it takes up to three to hide the latency
+// of a tile, so fewer are no cheaper), plus the parts' way through memory and the launch that joins them.  The rule's numbers were fitted to six shapes of 24 to 208
+// workgroups: 300 queries on 8400 keys, 8 heads: 21 parts 18.4 us, 33 parts 21.3, whole 96; one query of 8 images: 22 parts
+// 17 us, 32 parts 20.9.
+int attention_splits(long long workgroups, int tiles, long long rows, int resident)
 {
-    // up to about 4 workgroups for each of the 256 CUs, and at least `min_tiles` tiles for each part
-    const long long want = 1024 / workgroups, most = tiles / min_tiles;
-    const long long n = want < most ? want : most;
-    return n < 1 ? 1 : (int)n;
+    if (workgroups >= 512) return 1;
+    const float per_part = 0.1f + (float)rows / 5000.0f;
+    const long long least = resident < 3 ? resident : 3;
+    int best = 1;
+    float best_cost = INFINITY;
+    for (int k = 1; k <= tiles && k <= 256; ++k) {
+        const long long n = (workgroups * k + 255) / 256, last = n % resident;
+        const long long load = n - last + (last == 0 ? 0 : last > least ? last : least);
+        const float cost = (float)((tiles + k - 1) / k) * (float)load + (k > 1 ? per_part * (float)k + 12.0f : 0.0f);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = k;
+        }
+    }
+    return best;
 }
 
 namespace {
@@ -383,7 +404,7 @@ FwdPlan plan_forward(const yamd_attention_desc *d, bool biased)
     p.q_tiles = ceil_div(p.rows, kBlockRows);
     const int n_tiles = ceil_div(d->k_len, kTile);
     const long long wgs = (long long)d->batch * p.grid_heads * p.q_tiles;
-    const int splits = wgs >= 512 ? 1 : attention_splits(wgs, n_tiles, 4);
+    const int splits = attention_splits(wgs, n_tiles, (long long)d->batch * d->heads * d->q_len, p.dpad == 32 ? 4 : p.dpad == 64 ? 3 : 2);
     p.tiles_per_split = ceil_div(n_tiles, splits);
     p.splits = ceil_div(n_tiles, p.tiles_per_split);
     p.total = wgs * p.splits;
@@ -401,7 +422,9 @@ int launch_forward(const AttnFwdArgs &a, long long rows, hipStream_t st)
     hipLaunchKernelGGL((attention_kernel<D, BIAS, EXACT>), dim3(work_grid(a.total)), dim3(256), lds, st, a);
     YAMD_LAUNCH_CHECK();
     if (a.splits > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<D>), dim3(ceil_div(rows, 4)), dim3(256), 0, st, a, rows);
+        const long long lanes = rows * kJoinLanes<D>;
+        if (a.splits > 8) hipLaunchKernelGGL((attention_join_kernel<D, true>), dim3(ceil_div(rows * 64, 256)), dim3(256), 0, st, a, rows);
+        else hipLaunchKernelGGL((attention_join_kernel<D, false>), dim3(ceil_div(lanes, 256)), dim3(256), 0, st, a, rows);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;

@@ -169,8 +169,8 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
         const TileLoader<D, kBlockRows> vl(a.v.st, a.d, wave, lane);
         vl.load(smem + L::V, a.v.p + b * a.v.sb + kv_head * a.v.sh, tile * kBlockRows, a.k_len, wave, lane);
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     if (t0 < t1) fetch(t0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     TileReader<D> reader(lane);
     for (int t = t0; t < t1; ++t) {
         if constexpr (D > 64) reader.forget();
@@ -415,8 +415,8 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         clear_lds(smem, 2 * L::BUF);
         __syncthreads();
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     if (t0 < t1) fetch(t0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);                // (see the forward kernel)
     TileReader<D> reader(lane);
     for (int t = t0; t < t1; ++t) {
         if constexpr (D > 64) reader.forget();
@@ -636,10 +636,10 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     p.kv_tiles = ceil_div(d->k_len, kBlockRows);
     p.q_tiles = ceil_div(d->q_len, kBlockRows);
     const long long kw = bk * p.kv_tiles, qw = bh * p.q_tiles;
-    const int ks = kw >= 512 ? 1 : attention_splits(kw, qt, 4);
+    const int ks = attention_splits(kw, qt, 2 * bk * d->k_len, p.dpad == 32 ? 4 : 2);
     p.kv_loop = ceil_div(qt, ks);
     p.kv_splits = ceil_div(qt, p.kv_loop);
-    const int qs = biased || qw >= 512 ? 1 : attention_splits(qw, kt, 4);   // one owner per row of distances
+    const int qs = biased ? 1 : attention_splits(qw, kt, bh * d->q_len, p.dpad == 32 ? 3 : 2);   // one owner per row of distances
     p.q_loop = ceil_div(kt, qs);
     p.q_splits = ceil_div(kt, p.q_loop);
     p.kv_total = kw * p.kv_splits;
