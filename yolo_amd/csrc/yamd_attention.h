@@ -268,7 +268,7 @@ static inline AttnView view_of(const yamd_tokens *t) { return {(const __bf16 *)t
 
 // split of the looped axis when the owned rows alone give too few workgroups: the number of parts of `tiles` tiles, for
 // `rows` rows of results, with `resident` workgroups on a CU at a time (what their registers allow)
-int attention_splits(long long workgroups, int tiles, long long rows, int resident);
+int attention_splits(long long workgroups, int tiles, long long rows, int resident, float tile);
 
 // head width of the kernel that serves `d` channels: the channels beyond d are zeros in registers and LDS
 static inline int padded_head_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }

@@ -362,20 +362,21 @@ int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
 // Parts that the looped axis of `tiles` tiles is split into.  From 512 workgroups on there is nothing to gain (800 workgroups
 // of 100 tiles, d 64: 276 us whole, 284 in two parts; 832 of 25: 97 and 125).  Below, the cost in units of a tile's time
 // is that of a CU with n workgroups, `resident` at a time and each `steps` tiles long (it takes up to three to hide the latency
-// of a tile, so fewer are no cheaper), plus the parts' way through memory and the launch that joins them.  The rule's numbers were fitted to six shapes of 24 to 208
+// of a tile, so fewer are no cheaper), plus the parts' way through memory and the launch that joins them (`tile`: a tile's
+// time against the forward kernel's).  The rule's numbers were fitted to six shapes of 24 to 208
 // workgroups: 300 queries on 8400 keys, 8 heads: 21 parts 18.4 us, 33 parts 21.3, whole 96; one query of 8 images: 22 parts
 // 17 us, 32 parts 20.9.
-int attention_splits(long long workgroups, int tiles, long long rows, int resident)
+int attention_splits(long long workgroups, int tiles, long long rows, int resident, float tile)
 {
     if (workgroups >= 512) return 1;
-    const float per_part = 0.1f + (float)rows / 5000.0f;
+    const float per_part = (0.1f + (float)rows / 5000.0f) / tile, join = 12.0f / tile;
     const long long least = resident < 3 ? resident : 3;
     int best = 1;
     float best_cost = INFINITY;
     for (int k = 1; k <= tiles && k <= 256; ++k) {
         const long long n = (workgroups * k + 255) / 256, last = n % resident;
         const long long load = n - last + (last == 0 ? 0 : last > least ? last : least);
-        const float cost = (float)((tiles + k - 1) / k) * (float)load + (k > 1 ? per_part * (float)k + 12.0f : 0.0f);
+        const float cost = (float)((tiles + k - 1) / k) * (float)load + (k > 1 ? per_part * (float)k + join : 0.0f);
         if (cost < best_cost) {
             best_cost = cost;
             best = k;
@@ -404,7 +405,7 @@ FwdPlan plan_forward(const yamd_attention_desc *d, bool biased)
     p.q_tiles = ceil_div(p.rows, kBlockRows);
     const int n_tiles = ceil_div(d->k_len, kTile);
     const long long wgs = (long long)d->batch * p.grid_heads * p.q_tiles;
-    const int splits = attention_splits(wgs, n_tiles, (long long)d->batch * d->heads * d->q_len, p.dpad == 32 ? 4 : p.dpad == 64 ? 3 : 2);
+    const int splits = attention_splits(wgs, n_tiles, (long long)d->batch * d->heads * d->q_len, p.dpad == 32 ? 4 : p.dpad == 64 ? 3 : 2, 1.0f);
     p.tiles_per_split = ceil_div(n_tiles, splits);
     p.splits = ceil_div(n_tiles, p.tiles_per_split);
     p.total = wgs * p.splits;

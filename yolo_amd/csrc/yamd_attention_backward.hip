@@ -31,7 +31,7 @@ struct AttnBwdArgs {
     __bf16 *out0, *out1;           // dk, dv / dq
     long long o0_sb, o0_st, o0_sh, o1_sb, o1_st, o1_sh;
     float *part0, *part1;          // float32 parts [split][batch * heads][len][D] when splits > 1
-    float *part_bias;              // [batch * heads * tiles][part_len]: sums by distance of one workgroup
+    float *part_bias;              // [batch * heads * tiles * splits][part_len]: sums by distance of one workgroup
     int ring, part_len, window;
 };
 
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         cq = a.coord_last + map_coord(row0 + c32, a.map_w);    // (lanes beyond the queries too have distances of their own)
         c_first = a.coord_last + map_coord(tile * kBlockRows, a.map_w);
         c_last = a.coord_last + map_coord(last, a.map_w);
-        high = c_last + 1;                             // distances from here on are written out (a(0) = 0)
+        high = c_last - map_coord(split * a.loop_per_split * kTile, a.map_w) + 1;      // distances from here on are written out
         ring = rings + (2 * wave + half) * (a.ring + kRingPad);
         for (int e = tid; e < 8 * (a.ring + kRingPad); e += 256) rings[e] = 0.0f;
     }
@@ -395,10 +395,12 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
                         wave, lane);
         if (mp && wave == 0 && t * kTile + lane < a.k_len) mask_n = mp[t * kTile + lane];
     };
+    // coordinate of the last key that the workgroup walks
+    const int end_key = t1 * kTile < a.k_len ? t1 * kTile : a.k_len, coord_end = BIAS ? map_coord(end_key - 1, a.map_w) : 0;
     // writes the sums of the distances [low, high) out and clears them
     auto flush = [&](int low) {
         float *out = a.part_bias + (long long)wg * a.part_len;
-        const int base = c_first - a.coord_last;       // the smallest distance of the workgroup: first query, last key
+        const int base = c_first - coord_end;          // the smallest distance of the workgroup: first query, last key
         for (int e = low + tid; e < high; e += 256) {
             const int at = e & (a.ring - 1);
             float s = 0.0f;
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     }
     if (BIAS && a.part_bias) {
         __syncthreads();
-        flush(c_first - a.coord_last);
+        flush(c_first - coord_end);
     }
     if (row0 + c32 >= a.q_len) return;
     if (a.splits > 1) {
@@ -560,17 +562,20 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 }
 
 // Adds the workgroups' sums by distance: 64 distances x 16 threads per workgroup, thread y takes every 16th of a head's
-// (tile, image) pairs and a tree in LDS adds the sixteen.
+// (tile, split, image) triples and a tree in LDS adds the sixteen.
 __global__ __launch_bounds__(1024) void attention_bias_grad_kernel(AttnBwdArgs a, float *dbias)
 {
     __shared__ float part[16][64];
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6, off = blockIdx.x * 64 + x, head = blockIdx.y;
     float s = 0.0f;
-    for (int e = y; e < a.tiles * a.batch; e += 16) {
-        const int tile = e / a.batch, b = e - tile * a.batch;
+    for (int e = y; e < a.tiles * a.splits * a.batch; e += 16) {
+        const int b = e % a.batch, split = e / a.batch % a.splits, tile = e / a.batch / a.splits;
         const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
-        const int base = map_coord(tile * kBlockRows, a.map_w), n = map_coord(last, a.map_w) + a.coord_last - base + 1;
-        if (off >= base && off - base < n) s += a.part_bias[(((long long)b * a.heads + head) * a.tiles + tile) * a.part_len + off - base];
+        const int end = (split + 1) * a.loop_per_split * kTile < a.k_len ? (split + 1) * a.loop_per_split * kTile : a.k_len;
+        const int base = a.coord_last + map_coord(tile * kBlockRows, a.map_w) - map_coord(end - 1, a.map_w);
+        const int top = a.coord_last + map_coord(last, a.map_w) - map_coord(split * a.loop_per_split * kTile, a.map_w);
+        if (off >= base && off <= top)
+            s += a.part_bias[((((long long)b * a.heads + head) * a.tiles + tile) * a.splits + split) * a.part_len + off - base];
     }
     part[y][x] = s;
     __syncthreads();
@@ -636,10 +641,10 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     p.kv_tiles = ceil_div(d->k_len, kBlockRows);
     p.q_tiles = ceil_div(d->q_len, kBlockRows);
     const long long kw = bk * p.kv_tiles, qw = bh * p.q_tiles;
-    const int ks = attention_splits(kw, qt, 2 * bk * d->k_len, p.dpad == 32 ? 4 : 2);
+    const int ks = attention_splits(kw, qt, 2 * bk * d->k_len, p.dpad == 32 ? 4 : 2, 2.5f);
     p.kv_loop = ceil_div(qt, ks);
     p.kv_splits = ceil_div(qt, p.kv_loop);
-    const int qs = biased ? 1 : attention_splits(qw, kt, bh * d->q_len, p.dpad == 32 ? 3 : 2);   // one owner per row of distances
+    const int qs = attention_splits(qw, kt, bh * d->q_len, p.dpad == 32 ? 3 : 2, 2.5f);
     p.q_loop = ceil_div(kt, qs);
     p.q_splits = ceil_div(kt, p.q_loop);
     p.kv_total = kw * p.kv_splits;
@@ -651,9 +656,10 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     if (biased) {
         const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + 8 + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
         for (p.ring = 256; p.ring < span; p.ring *= 2) {}
-        const int coord_last = map_coord(d->k_len - 1, w);
-        p.part_len = coord_last + kBlockRows + (d->map_h > 1 ? kBlockRows + w : 0);
-        p.bias = up256((size_t)bh * p.q_tiles * p.part_len * sizeof(float));
+        // distances of one workgroup: 128 queries against the keys of its part
+        const int keys = p.q_loop * kTile < d->k_len ? p.q_loop * kTile : d->k_len;
+        p.part_len = keys + kBlockRows + (d->map_h > 1 ? keys + kBlockRows + 2 * w : 0);
+        p.bias = up256((size_t)p.q_total * p.part_len * sizeof(float));
     }
     p.workspace = p.delta + p.parts + p.bias;
     return p;
