@@ -390,7 +390,8 @@ int yamd_layer_norm_backward(const void *dy, long long dy_stride, const void *x,
                              long long rows, int c, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 /* bf16 tokens of several heads: channel c of head h of token t of image b is data[b*batch_stride + t*token_stride +
- * h*head_stride + c].  data is 16-byte aligned, strides are multiples of 8. */
+ * h*head_stride + c].  data is 16-byte aligned, strides are multiples of 8
+ * (token_stride at most 2^23). */
 typedef struct yamd_tokens {
     void *data;
     long long batch_stride, token_stride, head_stride;
@@ -401,7 +402,7 @@ typedef struct yamd_attention_desc {
     int32_t head_dim;                   /* multiple of 8, at most 128 */
     int32_t q_len, k_len;
     int32_t map_h, map_w;               /* with a bias: q_len == k_len == map_h * map_w, map_w <= 760 unless map_h == 1 */
-    float scale;                        /* > 0 */
+    float scale;                        /* 1e-20 to 1e20 */
 } yamd_attention_desc;
 
 /* o = softmax(scale q k^T + bias) v for each image and head.

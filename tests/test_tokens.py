@@ -124,7 +124,7 @@ def _attention(desc, bias=None, mask=None, mask_stride=100, ws=None, nb=0, exact
 
 @pytest.mark.parametrize("bad", [dict(batch=0), dict(heads=3), dict(kv_heads=0), dict(head_dim=4), dict(head_dim=12), dict(head_dim=136),
                                  dict(q_len=0), dict(k_len=0), dict(k_len=(1 << 24) + 1), dict(scale=0.0), dict(scale=-1.0),
-                                 dict(scale=math.inf), dict(scale=math.nan)])
+                                 dict(scale=math.inf), dict(scale=math.nan), dict(scale=1e-30)])
 def test_attention_abi_refuses_descriptors(bad):
     assert _attention(_desc(**bad)) == -1
     assert b"attention" in LIB.yamd_last_error()
@@ -134,7 +134,7 @@ def test_attention_abi_refuses_descriptors(bad):
 
 @pytest.mark.parametrize("name", ["q", "k", "v", "o"])
 @pytest.mark.parametrize("bad", [dict(data=None), dict(data=FAKE + 8), dict(token_stride=12), dict(token_stride=0), dict(head_stride=4),
-                                 dict(batch_stride=-8), dict(token_stride=(1 << 24) + 8)])
+                                 dict(batch_stride=-8), dict(token_stride=(1 << 23) + 8)])
 def test_attention_abi_refuses_tensors(name, bad):
     assert _attention(_desc(), **{name: _tokens(heads=4 if name in "qo" else 2, **bad)}) == -1
 

@@ -337,12 +337,13 @@ int check_attention(const yamd_attention_desc *d, const uint8_t *key_mask, long 
                  "attention: head_dim must be a multiple of 8 up to 128 (got %d)", d->head_dim);
     YAMD_REQUIRE(d->q_len <= (1 << 24) && d->k_len <= (1 << 24), "attention: more than 2^24 tokens (q %d, k %d)", d->q_len, d->k_len);
     YAMD_REQUIRE((long long)d->batch * d->heads <= (1 << 20), "attention: batch * heads = %lld above 2^20", (long long)d->batch * d->heads);
-    YAMD_REQUIRE(d->scale > 0.0f && d->scale < INFINITY, "attention: scale must be positive and finite (got %g)", (double)d->scale);
+    YAMD_REQUIRE(d->scale >= 1e-20f && d->scale <= 1e20f, "attention: scale must be between 1e-20 and 1e20 (got %g)", (double)d->scale);
     YAMD_REQUIRE(!key_mask || d->batch == 1 || mask_stride >= d->k_len, "attention: mask stride smaller than k_len");
     if (bias) {
         YAMD_REQUIRE(d->map_h > 0 && d->map_w > 0 && d->q_len == d->k_len && (long long)d->map_h * d->map_w == d->q_len,
                      "attention: a position bias needs q_len == k_len == map_h * map_w (got %d, %d, %d x %d)", d->q_len, d->k_len, d->map_h,
                      d->map_w);
+        YAMD_REQUIRE(d->heads <= 65535, "attention: a position bias for %d heads (at most 65535)", d->heads);
         YAMD_REQUIRE(d->map_h == 1 || d->map_w <= 760, "attention: a map of several rows is at most 760 wide (got %d x %d)", d->map_h, d->map_w);
     }
     return YAMD_OK;
@@ -355,7 +356,7 @@ int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
     YAMD_REQUIRE((d->batch == 1 || (t->batch_stride % 8 == 0 && t->batch_stride >= 0)) && (len == 1 || (t->token_stride % 8 == 0 && t->token_stride > 0)) &&
                      (heads == 1 || (t->head_stride % 8 == 0 && t->head_stride > 0)),
                  "attention: strides of %s must be positive multiples of 8 elements", name);
-    YAMD_REQUIRE(len == 1 || t->token_stride <= (1 << 24), "attention: tokens of %s are more than 2^24 elements apart", name);
+    YAMD_REQUIRE(len == 1 || t->token_stride <= (1 << 23), "attention: tokens of %s are more than 2^23 elements apart", name);
     return YAMD_OK;
 }
 

@@ -338,7 +338,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, std::optiona
     check_tokens(k, "k", dev, {b, lk, kv_heads, d});
     check_tokens(v, "v", dev, {b, lk, kv_heads, d});
     const double scale = scale_.value_or(1.0 / std::sqrt((double)d));
-    if (!((float)scale > 0.0f && (float)scale < INFINITY)) fail("scale must be positive and finite, got ", scale);
+    if (!(scale >= 1e-20 && scale <= 1e20)) fail("scale must be between 1e-20 and 1e20, got ", scale);
     if (mask.defined()) {
         require_gpu(mask, "key_mask", &dev);
         if (mask.scalar_type() != at::kBool || mask.dim() != 2 || mask.size(0) != b || mask.size(1) != lk || (lk > 1 && mask.stride(1) != 1) ||

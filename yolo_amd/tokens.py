@@ -88,7 +88,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     """``softmax(scale * q k^T + bias) v`` per image and head: (B, Lq, heads, d) bfloat16.
 
     q: (B, Lq, heads, d); k, v: (B, Lk, kv_heads, d), heads a multiple of kv_heads (consecutive heads share keys); bfloat16,
-    d a multiple of 8 up to 128.  scale: positive, 1/sqrt(d) by default.  key_mask: (B, Lk) bool, False = not attended (what
+    d a multiple of 8 up to 128.  scale: 1/sqrt(d) by default.  key_mask: (B, Lk) bool, False = not attended (what
     k and v hold there does not matter); a query left without keys gets zeros and no gradient.  bias: (heads,
     position.distances) float32, see ``relative_bias``, for self-attention over the h x w map (or sequence) of ``position``;
     values below -1e5 (-inf, the type's lowest value, ...) mask, and a query with only such scores is left without keys.
