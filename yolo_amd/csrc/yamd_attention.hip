@@ -374,14 +374,17 @@ int attention_splits(long long workgroups, int tiles, long long rows, int reside
     const long long least = resident < 3 ? resident : 3;
     int best = 1;
     float best_cost = INFINITY;
-    for (int k = 1; k <= tiles && k <= 256; ++k) {
+    for (int k = 1; k <= tiles && k <= 256;) {
+        const int steps = (tiles + k - 1) / k;
         const long long n = (workgroups * k + 255) / 256, last = n % resident;
         const long long load = n - last + (last == 0 ? 0 : last > least ? last : least);
-        const float cost = (float)((tiles + k - 1) / k) * (float)load + (k > 1 ? per_part * (float)k + join : 0.0f);
+        const float cost = (float)steps * (float)load + (k > 1 ? per_part * (float)k + join : 0.0f);
         if (cost < best_cost) {
             best_cost = cost;
             best = k;
         }
+        if (steps == 1) break;
+        k = (tiles + steps - 2) / (steps - 1);           // the next one with shorter parts: more parts of one length only cost more
     }
     return best;
 }
