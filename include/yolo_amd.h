@@ -403,7 +403,7 @@ typedef struct yamd_attention_desc {
     int32_t q_len, k_len;
     int32_t map_h, map_w;               /* with a bias: q_len == k_len == map_h * map_w, map_w <= 760 unless map_h == 1 */
     float scale;                        /* 1e-20 to 1e20 */
-} yamd_attention_desc;
+} yamd_attention_desc;                  /* batch * heads up to 2^20; batch * heads * q_len and batch * kv_heads * k_len up to 2^30 */
 
 /* o = softmax(scale q k^T + bias) v for each image and head.
  *   key_mask  (batch rows of k_len bytes, mask_stride apart; NULL = all): keys with 0 are not attended, and what k and v hold
@@ -420,7 +420,9 @@ int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const 
                    const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,
                    float *o_exact, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* Gradients of the above from o, lse and d_o; the probabilities are computed again.  dbias: one float per head and distance
- * (NULL: the bias has no gradient; otherwise o_exact is needed too).  Every sum is taken in a fixed order: equal inputs give equal bits. */
+ * (NULL: the bias has no gradient; otherwise o_exact is needed too).  Every sum is taken in a fixed order: equal inputs give equal bits.
+ * Rows of o, dq, dk and dv must not overlap.  With a bias the workspace holds a row of sums by distance for every 128 queries of
+ * a head, about q_len * k_len / 64 floats for a head of a map and half of that for a sequence. */
 size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *desc, int biased);
 int yamd_attention_backward(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
                             const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o, const float *o_exact,
@@ -428,7 +430,7 @@ int yamd_attention_backward(const yamd_attention_desc *desc, const yamd_tokens *
                             void *workspace, size_t workspace_bytes, void *stream);
 
 /* A position bias learned by buckets of distance: bias[head][i] = table[bucket_of[i]][head] for n_distances distances (a
- * bucket outside the table reads as NaN), and the gradient of the table, dtable[b][head] = sum of dbias[head][order[k]] over
+ * bucket outside the table reads as NaN; at most 2^20 buckets), and the gradient of the table, dtable[b][head] = sum of dbias[head][order[k]] over
  * start[b] <= k < start[b + 1].  `order` lists the distances by bucket, `start` has n_buckets + 1 entries. */
 int yamd_relative_bias(const void *table, int table_dtype, const int32_t *bucket_of, int n_distances, int heads, int n_buckets, float *bias,
                        void *stream);

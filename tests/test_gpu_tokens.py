@@ -151,6 +151,27 @@ def test_layer_norm_nan_and_constant_rows(gpu_device):
     assert torch.equal(y[keep], tokens.layer_norm(x[keep], eps=1e-5))
 
 
+def test_layer_norm_squares_that_overflow(gpu_device):
+    """A variance beyond float32 is infinite, and the row then comes out as its bias."""
+    x = torch.zeros(3, 96, device=gpu_device)
+    x[1, 5], x[2, 7] = 1e25, -3e15
+    b = torch.linspace(-1, 1, 96, device=gpu_device)
+    y = tokens.layer_norm(x, None, b)
+    assert torch.equal(y[0], b) and torch.equal(y[1], b)
+    want, tol = _norm_case(gpu_device, x[2:], None, b, 1e-5, torch.zeros_like(x[2:]), F)
+    _within("y", y[2:], want[0], tol[0])
+
+
+def test_layer_norm_without_rows(gpu_device):
+    for params in (False, True):
+        x = torch.zeros(0, 40, device=gpu_device, dtype=torch.bfloat16, requires_grad=True)
+        w = torch.ones(40, device=gpu_device, requires_grad=True) if params else None
+        y = tokens.layer_norm(x, w, w)
+        assert torch.autograd.grad(y, x, torch.zeros_like(y), retain_graph=True)[0].shape == (0, 40)
+        if params:
+            assert torch.equal(torch.autograd.grad(y, w, torch.zeros_like(y))[0], torch.zeros(40, device=gpu_device))
+
+
 def test_layer_norm_rows_beyond_32_bits(gpu_device):
     """Rows 2^30 elements apart: the third starts beyond 2^31."""
     big = torch.empty(2 * (1 << 30) + 64, dtype=torch.bfloat16, device=gpu_device)
@@ -410,6 +431,17 @@ def test_attention_layouts(gpu_device):
     assert torch.equal(torch.autograd.grad(o.float().sum(), parts, retain_graph=True)[0], torch.autograd.grad(o, parts, torch.ones_like(o), retain_graph=True)[0])
     do_t = do.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
     assert torch.equal(torch.autograd.grad(o, parts, do_t)[2], want[2])
+
+
+def test_attention_gradient_from_a_longer_vector(gpu_device):
+    """The gradient of a result that was joined to something else starts anywhere."""
+    leaves, do, _ = _inputs(gpu_device, 77, 1, 33, 65, 2, 1, 32)
+    want = torch.autograd.grad(tokens.attention(*leaves), leaves, do)
+    flat = torch.cat([torch.zeros(3, device=gpu_device, dtype=torch.bfloat16), do.flatten()])
+    joined = flat[3:].view(do.shape)
+    assert joined.data_ptr() % 16 and joined.is_contiguous()
+    got = torch.autograd.grad(tokens.attention(*leaves), leaves, joined)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_attention_broadcast_batch_is_refused(gpu_device):

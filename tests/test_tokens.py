@@ -35,7 +35,15 @@ def test_axis_buckets(buckets, far):
     assert b[-1] == buckets - 1 and b[0] == half - 1
 
 
+def test_axis_buckets_far_distance_costs_nothing():
+    """Distances that the axis does not have are not searched."""
+    assert tokens.axis_buckets(9, 8, 10 ** 12) == [min(m, 2) for m in range(8, 0, -1)] + [0] + \
+        [4 + min(m, 2) for m in range(1, 9)]
+
+
 def test_axis_buckets_refuses():
+    with pytest.raises(L.YamdError):
+        tokens.axis_buckets(0, 8, 16)
     for buckets, far in [(6, 16), (0, 16), (8, 2), (-4, 3)]:
         with pytest.raises(L.YamdError):
             tokens.axis_buckets(5, buckets, far)
@@ -61,6 +69,8 @@ def test_relative_position_refuses():
     for h, w in [(0, 5), (2, 761), (5000, 5000)]:
         with pytest.raises(L.YamdError):
             tokens.RelativePosition(h, w, 8, 16, device="cpu")
+    with pytest.raises(L.YamdError):
+        tokens.RelativePosition(4, 4, 1028, 2000, device="cpu")            # 1028^2 rows
     assert tokens.RelativePosition(1, 2000, 8, 16, device="cpu").distances == 3999
 
 
@@ -137,6 +147,28 @@ def test_attention_abi_refuses_descriptors(bad):
                                  dict(batch_stride=-8), dict(token_stride=(1 << 23) + 8)])
 def test_attention_abi_refuses_tensors(name, bad):
     assert _attention(_desc(), **{name: _tokens(heads=4 if name in "qo" else 2, **bad)}) == -1
+
+
+@pytest.mark.parametrize("bad", [dict(token_stride=8), dict(token_stride=248), dict(head_stride=8), dict(head_stride=56), dict(batch_stride=0),
+                                 dict(batch_stride=25592), dict(token_stride=64, head_stride=6392)])
+def test_attention_abi_refuses_results_that_overlap(bad):
+    """Inputs may repeat memory, results may not; (batch, head, token) order is as good as (batch, token, head)."""
+    r, d, ok, kv = ctypes.byref, _desc(), _tokens(), _tokens(heads=2)
+    assert _attention(d, o=_tokens(**bad)) == -1 and b"overlap" in LIB.yamd_last_error()
+    back = lambda dq=ok, dk=kv, dv=kv: LIB.yamd_attention_backward(r(d), r(ok), r(kv), r(kv), None, 0, None, r(ok), None, FAKE, r(ok), r(dq), r(dk),
+                                                                   r(dv), None, None, 0, None)
+    assert back(dq=_tokens(**bad)) == -1 and b"overlap" in LIB.yamd_last_error()
+    for two in (dict(token_stride=8), dict(token_stride=120), dict(batch_stride=0)):
+        assert back(dk=_tokens(heads=2, **two)) == -1 and back(dv=_tokens(heads=2, **two)) == -1 and b"overlap" in LIB.yamd_last_error()
+    heads_first = _tokens(token_stride=64, head_stride=6400)
+    assert back(dq=heads_first) == -3                                            # all that is missing is the workspace
+
+
+def test_attention_abi_refuses_sizes_beyond_a_launch():
+    for k in (dict(batch=1 << 10, heads=1 << 10, kv_heads=1 << 10, q_len=1025, k_len=1), dict(batch=1 << 10, heads=1 << 10, kv_heads=1 << 10, k_len=1025)):
+        assert _attention(_desc(**k)) == -1 and b"2^30" in LIB.yamd_last_error()
+        assert LIB.yamd_attention_backward_workspace_bytes(ctypes.byref(_desc(**k)), 0) == 0
+    assert LIB.yamd_relative_bias_backward(FAKE, FAKE, FAKE, 9, 2, (1 << 20) + 1, FAKE, 0, None) == -1
 
 
 def test_attention_abi_refuses_bias_mask_workspace():

@@ -264,6 +264,7 @@ static inline int window_len(int map_h, int map_w)
 // argument checks shared by both directions (yamd_attention.hip)
 int check_attention(const yamd_attention_desc *d, const uint8_t *key_mask, long long mask_stride, const float *bias);
 int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, int heads, const char *name);
+int check_result(const yamd_attention_desc *d, const yamd_tokens *t, int len, int heads, const char *name);
 static inline AttnView view_of(const yamd_tokens *t) { return {(const __bf16 *)t->data, t->batch_stride, t->token_stride, t->head_stride}; }
 
 // split of the looped axis when the owned rows alone give too few workgroups: the number of parts of `tiles` tiles, for

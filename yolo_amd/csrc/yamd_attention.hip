@@ -16,6 +16,7 @@
 // keys are split over workgroups whose float32 parts a second kernel joins.
 #include "yamd_attention.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace yamd {
@@ -337,6 +338,9 @@ int check_attention(const yamd_attention_desc *d, const uint8_t *key_mask, long 
                  "attention: head_dim must be a multiple of 8 up to 128 (got %d)", d->head_dim);
     YAMD_REQUIRE(d->q_len <= (1 << 24) && d->k_len <= (1 << 24), "attention: more than 2^24 tokens (q %d, k %d)", d->q_len, d->k_len);
     YAMD_REQUIRE((long long)d->batch * d->heads <= (1 << 20), "attention: batch * heads = %lld above 2^20", (long long)d->batch * d->heads);
+    // (a launch has fewer than 2^32 threads; workgroups take 128 rows or a head each)
+    YAMD_REQUIRE((long long)d->batch * d->heads * d->q_len <= (1 << 30) && (long long)d->batch * d->kv_heads * d->k_len <= (1 << 30),
+                 "attention: more than 2^30 rows (batch %d, heads %d of %d, q %d, k %d)", d->batch, d->kv_heads, d->heads, d->q_len, d->k_len);
     YAMD_REQUIRE(d->scale >= 1e-20f && d->scale <= 1e20f, "attention: scale must be between 1e-20 and 1e20 (got %g)", (double)d->scale);
     YAMD_REQUIRE(!key_mask || d->batch == 1 || mask_stride >= d->k_len, "attention: mask stride smaller than k_len");
     if (bias) {
@@ -357,6 +361,26 @@ int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
                      (heads == 1 || (t->head_stride % 8 == 0 && t->head_stride > 0)),
                  "attention: strides of %s must be positive multiples of 8 elements", name);
     YAMD_REQUIRE(len == 1 || t->token_stride <= (1 << 23), "attention: tokens of %s are more than 2^23 elements apart", name);
+    return YAMD_OK;
+}
+
+// rows of a result must not share memory: taken from the shortest stride on, each axis steps over all that the ones before span
+int check_result(const yamd_attention_desc *d, const yamd_tokens *t, int len, int heads, const char *name)
+{
+    const int rc = check_tokens(d, t, len, heads, name);
+    if (rc != YAMD_OK) return rc;
+    struct Axis {
+        long long stride;
+        int n;
+    } axis[3] = {{t->head_stride, heads}, {t->token_stride, len}, {t->batch_stride, d->batch}};
+    std::sort(axis, axis + 3, [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+    long long span = d->head_dim;
+    for (const Axis &x : axis) {
+        if (x.n == 1) continue;
+        YAMD_REQUIRE(x.stride >= span, "attention: rows of %s overlap (strides %lld, %lld, %lld)", name, t->batch_stride, t->token_stride,
+                     t->head_stride);
+        span += x.stride * (x.n - 1);
+    }
     return YAMD_OK;
 }
 
@@ -462,11 +486,10 @@ extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q
     if (rc == YAMD_OK) rc = check_tokens(d, q, d->q_len, d->heads, "q");
     if (rc == YAMD_OK) rc = check_tokens(d, k, d->k_len, d->kv_heads, "k");
     if (rc == YAMD_OK) rc = check_tokens(d, v, d->k_len, d->kv_heads, "v");
-    if (rc == YAMD_OK) rc = check_tokens(d, o, d->q_len, d->heads, "o");
+    if (rc == YAMD_OK) rc = check_result(d, o, d->q_len, d->heads, "o");
     if (rc != YAMD_OK) return rc;
     YAMD_REQUIRE(!o_exact || (bias && ((uintptr_t)o_exact & 15) == 0), "attention: o_exact goes with a bias and is 16-byte aligned");
     const FwdPlan p = plan_forward(d, bias != nullptr);
-    YAMD_REQUIRE(p.total <= (1ll << 30), "attention: %lld workgroups", p.total);
     if (p.workspace && (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15))) {
         set_error("attention: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace ? workspace_bytes : (size_t)0, p.workspace);
         return YAMD_ENOSPC;

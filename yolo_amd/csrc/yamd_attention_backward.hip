@@ -46,10 +46,9 @@ constexpr int kMostRing = 2048;                // positions for the widest map (
 __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
 {
     const long long rows = (long long)a.batch * a.heads * a.q_len;
-    const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
     const int c = (threadIdx.x & 15) * 8;
-    float s = 0.0f;
-    if (at < rows) {
+    for (long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); at < rows; at += (long long)gridDim.x * 16) {
+        float s = 0.0f;
         // rows in the order (batch, token, head), which is the order in memory of the usual layout
         const int head = (int)(at % a.heads), i = (int)(at / a.heads % a.q_len);
         const long long b = at / a.heads / a.q_len;
@@ -671,7 +670,7 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
     if (rc == YAMD_OK) rc = QAttr::ensure();
     if (rc != YAMD_OK) return rc;
     const long long rows = (long long)a.batch * a.heads * a.q_len;
-    hipLaunchKernelGGL(attention_delta_kernel, dim3(ceil_div(rows, 16)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(attention_delta_kernel, dim3(ceil_div(rows < (1 << 24) ? rows : 1 << 24, 16)), dim3(256), 0, st, a);
     YAMD_LAUNCH_CHECK();
 
     AttnBwdArgs w = a;
@@ -743,15 +742,14 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     if (rc == YAMD_OK) rc = check_tokens(d, v, d->k_len, d->kv_heads, "v");
     if (rc == YAMD_OK) rc = check_tokens(d, o, d->q_len, d->heads, "o");
     if (rc == YAMD_OK) rc = check_tokens(d, d_o, d->q_len, d->heads, "do");
-    if (rc == YAMD_OK) rc = check_tokens(d, dq, d->q_len, d->heads, "dq");
-    if (rc == YAMD_OK) rc = check_tokens(d, dk, d->k_len, d->kv_heads, "dk");
-    if (rc == YAMD_OK) rc = check_tokens(d, dv, d->k_len, d->kv_heads, "dv");
+    if (rc == YAMD_OK) rc = check_result(d, dq, d->q_len, d->heads, "dq");
+    if (rc == YAMD_OK) rc = check_result(d, dk, d->k_len, d->kv_heads, "dk");
+    if (rc == YAMD_OK) rc = check_result(d, dv, d->k_len, d->kv_heads, "dv");
     if (rc != YAMD_OK) return rc;
     YAMD_REQUIRE(lse, "attention backward: lse is null");
     YAMD_REQUIRE(!dbias || bias, "attention backward: a bias gradient without a bias");
     YAMD_REQUIRE(!dbias || (o_exact && ((uintptr_t)o_exact & 15) == 0), "attention backward: a bias gradient needs o_exact (16-byte aligned)");
     const BwdPlan p = plan_backward(d, bias != nullptr);
-    YAMD_REQUIRE(p.kv_total <= (1ll << 30) && p.q_total <= (1ll << 30), "attention backward: too many workgroups");
     if (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15)) {
         set_error("attention backward: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace ? workspace_bytes : (size_t)0, p.workspace);
         return YAMD_ENOSPC;

@@ -80,10 +80,11 @@ __device__ __forceinline__ void load_params(const void *p, int bf16, const int (
     }
 }
 
-// 1 / sqrt(t): the instruction's result (1 ulp) and one Newton step; t below its range (eps = 0 only) the long way
+// 1 / sqrt(t): the instruction's result (1 ulp) and one Newton step; t beyond its range (eps = 0, or squares near the end of
+// float32; of an overflow 0, not the step's inf * 0) the long way
 __device__ __forceinline__ float inverse_sqrt(float t)
 {
-    if (t < 1e-30f) return 1.0f / sqrtf(t);
+    if (t < 1e-30f || t > 1e30f) return 1.0f / sqrtf(t);
     const float r = __builtin_amdgcn_rsqf(t);
     return r * (1.5f - 0.5f * t * r * r);
 }

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void relative_bias_backward_kernel(const float
 int check_bias(int dtype, int n, int heads, int buckets)
 {
     YAMD_REQUIRE(dtype == YAMD_F32 || dtype == YAMD_BF16, "relative bias: unknown dtype %d", dtype);
-    YAMD_REQUIRE(n > 0 && n <= (1 << 27) && heads > 0 && heads <= 65535 && buckets > 0 && buckets <= (1 << 24),
+    YAMD_REQUIRE(n > 0 && n <= (1 << 27) && heads > 0 && heads <= 65535 && buckets > 0 && buckets <= (1 << 20),
                  "relative bias: bad shape distances=%d heads=%d buckets=%d", n, heads, buckets);
     return YAMD_OK;
 }

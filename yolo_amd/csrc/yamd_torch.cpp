@@ -135,6 +135,7 @@ struct LayerNorm : Function<LayerNorm> {
         // (absent tensors have no edge)
         if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty_like(w);
         if (b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty_like(b);
+        if (n == 0 && !dw.defined() && !db.defined()) return {dx, Tensor(), Tensor(), Tensor()};
         size_t nbytes = 0;
         if (dw.defined() || db.defined()) {
             nbytes = yamd_layer_norm_backward_workspace_bytes(n, (int)c);
@@ -294,7 +295,8 @@ struct Attention : Function<Attention> {
         Tensor dq = result(q), dk = result(k), dv = result(v), dbias;
         if (bias.defined() && ctx->needs_input_grad(3)) dbias = result(bias);
         if (!nothing) {
-            const Tensor go = grads[0].contiguous();
+            Tensor go = grads[0].contiguous();
+            if (reinterpret_cast<uintptr_t>(go.data_ptr()) % 16) go = go.clone();      // (a piece of a longer vector)
             const yamd_attention_desc d = descriptor(q, k, ctx->saved_data["scale"].toDouble(), ctx->saved_data["h"].toInt(),
                                                      ctx->saved_data["w"].toInt());
             const yamd_tokens tq = tokens(q), tk = tokens(k), tv = tokens(v), to = tokens(o), tg = tokens(go), tdq = tokens(dq), tdk = tokens(dk),

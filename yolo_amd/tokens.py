@@ -28,6 +28,8 @@ def axis_buckets(n: int, buckets: int, max_distance: int) -> List[int]:
     """Bucket of each signed distance -(n - 1) .. n - 1 along one axis.  Half of the ``buckets`` go to positive distances; of
     a half, the first half hold one distance each and the others grow by a constant factor up to ``max_distance``, the last
     one holding all that is farther.  Decided by whole-number comparisons, so a border falls on one side everywhere."""
+    if n < 1:
+        raise _lib.YamdError(f"an axis has at least one position, got {n}")
     if buckets < 4 or buckets % 4:
         raise _lib.YamdError(f"buckets must be a positive multiple of 4, got {buckets}")
     half, near = buckets // 2, buckets // 4
@@ -37,7 +39,7 @@ def axis_buckets(n: int, buckets: int, max_distance: int) -> List[int]:
     # first distance of bucket near + t: the smallest m with (m / near)^steps >= (max_distance / near)^t
     first, m = [], near
     for t in range(steps):
-        while m ** steps * near ** t < near ** steps * max_distance ** t:
+        while m < n and m ** steps * near ** t < near ** steps * max_distance ** t:      # (n: beyond the axis)
             m += 1
         first.append(m)
     mag = []
@@ -62,6 +64,8 @@ class RelativePosition:
         if h > 1 and w > 760:
             raise _lib.YamdError(f"a map of several rows is at most 760 wide, got {h} x {w}")
         self.h, self.w, self.buckets, self.max_distance = int(h), int(w), int(buckets), int(max_distance)
+        if buckets ** (2 if h > 1 else 1) > 1 << 20:
+            raise _lib.YamdError(f"more than 2^20 rows in the table of {buckets} buckets")
         of = torch.tensor(axis_buckets(w, buckets, max_distance), dtype=torch.int64)
         self.rows = buckets
         if h > 1:
@@ -88,7 +92,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     """``softmax(scale * q k^T + bias) v`` per image and head: (B, Lq, heads, d) bfloat16.
 
     q: (B, Lq, heads, d); k, v: (B, Lk, kv_heads, d), heads a multiple of kv_heads (consecutive heads share keys); bfloat16,
-    d a multiple of 8 up to 128.  scale: 1/sqrt(d) by default.  key_mask: (B, Lk) bool, False = not attended (what
+    d a multiple of 8 up to 128, channels contiguous and rows at multiples of 16 bytes (copy a broadcast tensor first).  scale: 1/sqrt(d) by default.  key_mask: (B, Lk) bool, False = not attended (what
     k and v hold there does not matter); a query left without keys gets zeros and no gradient.  bias: (heads,
     position.distances) float32, see ``relative_bias``, for self-attention over the h x w map (or sequence) of ``position``;
     values below -1e5 (-inf, the type's lowest value, ...) mask, and a query with only such scores is left without keys.
