@@ -410,11 +410,13 @@ typedef struct yamd_attention_desc {
  *             there does not matter.  A query that is left without keys gets zeros.
  *   bias      (heads rows of (2 map_h - 1)(2 map_w - 1) floats; NULL = none): added to the score of a query at (y, x) and a
  *             key at (y', x') from [(y - y' + map_h - 1)(2 map_w - 1) + x - x' + map_w - 1].  Biases below -1e5 (-inf, the
- *             type's lowest value, ...) mask: a query with only such scores counts as left without keys.
+ *             type's lowest value, ...) mask: a query with only such scores counts as left without keys (so with a bias the
+ *             largest score of a query that has keys must lie above -1e5).
  *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted; only with a bias): o before its
  *             rounding to bf16 and with probabilities kept to 16 bits, which the gradient of a bias needs.
  *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
- * The workspace (16-byte aligned; 0 bytes for most shapes) holds parts of o where the keys are split over workgroups. */
+ * Results must not overlap operands.  The workspace (16-byte aligned; 0 bytes for most shapes) holds parts of o where the keys
+ * are split over workgroups. */
 size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biased);
 int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
                    const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,

@@ -230,6 +230,13 @@ def test_program_records_tokens():
                         (qkv.slice(0, 64), qkv.slice(64, 64), qkv.slice(128, 64), dict(heads=2, position=pos))]:
         with pytest.raises(L.YamdError):
             p.attention("bad", q, k, v, **kw)
+    fp32, wide = p.buffer(8, 8, 64, torch.float32), p.buffer(8, 8, 72)
+    for x, out in [(fp32, None), (x, fp32)]:
+        with pytest.raises(L.YamdError):
+            p.layer_norm("bad", x, None, None, out=out)
+    for out in (fp32, wide.slice(4, 64), qkv.slice(128, 64), qkv.slice(96, 64)):
+        with pytest.raises(L.YamdError):
+            p.attention("bad", qkv.slice(0, 64), qkv.slice(64, 64), qkv.slice(128, 64), 2, out=out)
 
 
 def test_plan_takes_token_ops_and_refuses_beyond():

@@ -447,6 +447,8 @@ class Program:
         if out is None:
             out = self.buffer(x.h, x.w, x.c)
         assert (out.h, out.w, out.c) == (x.h, x.w, x.c), (name, out, x)
+        if any(self.buffers[t.buf][3] != torch.bfloat16 for t in (x, out)):
+            raise _lib.YamdError(f"layer_norm[{name}]: maps must be bf16")
         layer = NormLayer(name, weight, bias, eps)
         self.stems.append(layer)                            # (uploaded with the other layers)
         self.ops.append(("norm", layer, x, out))
@@ -471,6 +473,10 @@ class Program:
         if out is None:
             out = self.buffer(q.h, q.w, q.c)
         assert (out.h, out.w, out.c) == (q.h, q.w, q.c), (name, out, q)
+        if self.buffers[out.buf][3] != torch.bfloat16 or out.coff % 8 or self.buffers[out.buf][2] % 8:
+            raise _lib.YamdError(f"attention[{name}]: the result must be a bf16 map whose channels start at a multiple of 8")
+        if any(t.buf == out.buf and t.coff < out.coff + out.c and out.coff < t.coff + t.c for t in (q, k, v)):
+            raise _lib.YamdError(f"attention[{name}]: the result overlaps an operand")
         layer = AttentionLayer(name, heads, kv_heads, d, (q.h, q.w), k.h * k.w, 1.0 / d ** 0.5 if scale is None else float(scale), table, position)
         layer.workspace = f"workspace {len(self.ops)} of {name}"
         self.stems.append(layer)

@@ -4,7 +4,9 @@ A map's NHWC pixels are its tokens: a (B, H, W, C) activation is ``(B, H*W, head
 a channel slice of a wider buffer.  Tensors live on the GPU; attention takes bfloat16, layer norm bfloat16 or float32 rows.
 Gradients flow through ``torch.autograd`` (once: the gradients carry no graph of their own); all arithmetic happens inside
 libyolo_amd.so, on torch's current stream of the tensors' device, and equal inputs give equal bits.  Results and scratch are
-torch allocations of each call, so calls on different streams, or captured into different graphs, share nothing.
+torch allocations of each call, so calls on different streams, or captured into different graphs, share nothing.  A training
+step that is captured into a graph takes its forward and backward pass together; no eager result of the same leaves may be
+alive meanwhile (autograd would tie the captured stream to the eager one).
 ``engine.Program`` records the forward passes into a layer program.
 """
 from typing import List, Optional
@@ -95,7 +97,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     d a multiple of 8 up to 128, channels contiguous and rows at multiples of 16 bytes (copy a broadcast tensor first).  scale: 1/sqrt(d) by default.  key_mask: (B, Lk) bool, False = not attended (what
     k and v hold there does not matter); a query left without keys gets zeros and no gradient.  bias: (heads,
     position.distances) float32, see ``relative_bias``, for self-attention over the h x w map (or sequence) of ``position``;
-    values below -1e5 (-inf, the type's lowest value, ...) mask, and a query with only such scores is left without keys.
+    values below -1e5 (-inf, the type's lowest value, ...) mask, and a query with only such scores is left without keys
+    (with a bias, the largest score of a query that has keys must lie above -1e5).
     Scores, statistics and sums are float32; probabilities are rounded to bfloat16 for the products with v and do, and score
     gradients for the products with q and k."""
     if (bias is None) != (position is None):
