@@ -415,7 +415,7 @@ typedef struct yamd_attention_desc {
  *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted; only with a bias): o before its
  *             rounding to bf16 and with probabilities kept to 16 bits, which the gradient of a bias needs.
  *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
- * Results must not overlap operands.  The workspace (16-byte aligned; 0 bytes for most shapes) holds parts of o where the keys
+ * Results must not overlap operands.  The workspace (16-byte aligned; may need no bytes) holds parts of o where the keys
  * are split over workgroups. */
 size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biased);
 int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,

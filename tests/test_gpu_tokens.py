@@ -343,6 +343,23 @@ def test_attention_with_learned_bias(gpu_device, b, h, w, heads, d, buckets, tdt
     _within("dtable", dt, dwant, dtol + (U if tdtype == torch.bfloat16 else F) * (dwant.abs() + dtol))
 
 
+@pytest.mark.parametrize("lq,lk,heads,d", [(1600, 1600, 20, 32), (130, 1500, 129, 64), (1664, 70, 20, 128), (100, 2000, 257, 96)])
+def test_attention_cuts_the_last_items_only(gpu_device, lq, lk, heads, d):
+    """A little more than 256 tiles of rows: 256 walk their keys (queries) whole, the others in parts."""
+    (q, k, v), do, g = _inputs(gpu_device, lq + lk, 1, lq, lk, heads, heads, d)
+    mask = torch.rand(1, lk, generator=g, device=gpu_device) < 0.9
+    mask[0, lk // 3:lk // 2] = False
+    _check(gpu_device, q, k, v, do, mask=mask)
+
+
+@pytest.mark.parametrize("b,h,w,heads,d", [(1, 40, 40, 20, 32), (2, 1, 1000, 17, 64), (3, 25, 30, 15, 128)])
+def test_biased_attention_cuts_the_last_items_only(gpu_device, b, h, w, heads, d):
+    (q, k, v), do, g = _inputs(gpu_device, h * w + d, b, h * w, h * w, heads, heads, d)
+    pos = tokens.RelativePosition(h, w, 16, 64, gpu_device)
+    table = torch.randn(pos.rows, heads, generator=g, device=gpu_device).requires_grad_()
+    _check(gpu_device, q, k, v, do, table=table, pos=pos)
+
+
 def test_bias_that_masks(gpu_device):
     """-inf, the lowest value and usual large negative values in the bias mask; rows that have nothing else get zeros."""
     h, w, heads = 4, 40, 2

@@ -114,14 +114,45 @@ __device__ __forceinline__ float with_other_half(float v, F f)
     return f(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
-// Workgroup ids go round-robin to the 8 XCDs: give each a contiguous range of the work, so that the workgroups that share
-// one head's keys share an L2.  Returns a value >= total for the ids beyond the work.
-__device__ __forceinline__ int work_item()
+// How the tiles of owned rows (items) become workgroups: the first `whole` items walk the looped axis from end to end, each
+// of the `rest` behind them is cut into `splits` parts of `per_split` steps, a workgroup each, whose float32 results another
+// kernel joins.
+struct WorkSplit {
+    int whole, rest, splits, per_split;
+    int tile_rows;                       // rows of an item: 128, or all when there are fewer
+    __host__ __device__ int whole_grid() const { return (whole + 7) / 8 * 8; }
+    int grid() const { return whole_grid() + (rest * splits + 7) / 8 * 8; }
+    __host__ __device__ int part_rows() const { return rest * tile_rows; }       // (of one part each: rest < 256)
+};
+struct Piece {
+    int item, split;                     // split < 0: all of the item
+    int t0, t1;                          // steps
+    int index;                           // among all pieces
+};
+// The workgroup's piece; false for the ids beyond the work.  Workgroup ids go round-robin to the 8 XCDs: each gets a contiguous
+// range of the items, so that the workgroups that share one head's keys share an L2.
+__device__ __forceinline__ bool work_piece(const WorkSplit &w, int steps, Piece &p)
 {
-    const int per_xcd = gridDim.x >> 3;
-    return (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    const int grid0 = w.whole_grid(), part = blockIdx.x >= grid0;
+    const int id = part ? blockIdx.x - grid0 : blockIdx.x, per_xcd = (part ? gridDim.x - grid0 : grid0) >> 3;
+    const int at = (id & 7) * per_xcd + (id >> 3);
+    if (!part) {
+        p = {at, -1, 0, steps, at};
+        return at < w.whole;
+    }
+    const int of = __builtin_amdgcn_readfirstlane(at / w.splits);
+    p.item = w.whole + of;
+    p.split = at - of * w.splits;
+    p.t0 = p.split * w.per_split;
+    p.t1 = p.t0 + w.per_split < steps ? p.t0 + w.per_split : steps;
+    p.index = w.whole + at;
+    return at < w.rest * w.splits;
 }
-static inline int work_grid(long long total) { return (int)(ceil_div(total, 8) * 8); }
+// row of a part's results: parts are laid out [split][item of the rest][row of the item]
+__device__ __forceinline__ int part_row(const WorkSplit &w, const Piece &p, int row)
+{
+    return (p.split * w.rest + p.item - w.whole) * w.tile_rows + row;
+}
 
 // A position t of a map of width w at (t / w, t % w) has the coordinate a(t) = (t / w)(2 w - 1) + t % w, and the distance of
 // two positions the index a(query) - a(key) + a(last) among the (2 h - 1)(2 w - 1) distances of the map.
@@ -267,9 +298,9 @@ int check_tokens(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
 int check_result(const yamd_attention_desc *d, const yamd_tokens *t, int len, int heads, const char *name);
 static inline AttnView view_of(const yamd_tokens *t) { return {(const __bf16 *)t->data, t->batch_stride, t->token_stride, t->head_stride}; }
 
-// split of the looped axis when the owned rows alone give too few workgroups: the number of parts of `tiles` tiles, for
-// `rows` rows of results, with `resident` workgroups on a CU at a time (what their registers allow)
-int attention_splits(long long workgroups, int tiles, long long rows, int resident, float tile);
+// the split of `items` items (tiles of an axis of `len` rows) of `steps` steps each, with `resident` workgroups on a CU at a time (what their registers allow),
+// `results` results per row, and a step of `step` times the forward kernel's duration
+WorkSplit split_work(long long items, int steps, int len, int resident, int results, float step);
 
 // head width of the kernel that serves `d` channels: the channels beyond d are zeros in registers and LDS
 static inline int padded_head_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }

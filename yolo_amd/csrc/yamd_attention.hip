@@ -32,9 +32,10 @@ struct AttnFwdArgs {
     const float *bias;             // [heads][(2 h - 1)(2 w - 1)]
     int n_off, coord_last, map_w, window;
     int batch, q_len, k_len, d, heads, kv_heads, group;
-    int packed, rows, q_tiles, grid_heads, splits, tiles_per_split, total;
+    int packed, rows, q_tiles, grid_heads;
+    WorkSplit split;
     float scale;
-    float *part_o, *part_ml;       // [split][batch heads][q_len][D] and [...][2] when splits > 1
+    float *part_o, *part_ml;       // results of parts: [part row][D] and [part row][2]
 };
 
 // LDS: two buffers of a tile of keys and one of values; then the coordinates and the mask of the two tiles' rows, and two
@@ -46,19 +47,15 @@ struct FwdLds {
 };
 
 template <int D, int BIAS, bool EXACT>
-__global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
+__global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attention_kernel(AttnFwdArgs a)
 {
     using L = FwdLds<D>;
     constexpr int NKS = D / 16, NB = D / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
-    int item = work_item();
-    if (item >= a.total) return;
-    const int split = item % a.splits;
-    item /= a.splits;
-    const int q_tile = item % a.q_tiles;
-    item /= a.q_tiles;
-    const int gh = item % a.grid_heads, b = item / a.grid_heads;
+    Piece piece;
+    if (!work_piece(a.split, (a.k_len + kTile - 1) / kTile, piece)) return;
+    const int q_tile = piece.item % a.q_tiles, gh = piece.item / a.q_tiles % a.grid_heads, b = piece.item / a.q_tiles / a.grid_heads;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int row0 = q_tile * kBlockRows + wave * 32;
@@ -88,8 +85,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
     float m = -INFINITY, l = 0.0f;                       // running maximum (units of log 2) and this half's sum
     const float c2 = a.scale * kLog2e;
 
-    const int t0 = split * a.tiles_per_split, n_tiles = (a.k_len + kTile - 1) / kTile;
-    const int t1 = t0 + a.tiles_per_split < n_tiles ? t0 + a.tiles_per_split : n_tiles;
+    const int t0 = piece.t0, t1 = piece.t1;
 
     // distance index = c_row - a(key); a window starts at the distance of the workgroup's first row and the tile's last key
     const float *bias = BIAS ? a.bias + (long long)gh * a.n_off : nullptr;
@@ -231,8 +227,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
     }
     l = with_other_half(l, [](float x, float y) { return x + y; });
     if (row0 + c32 >= a.rows) return;
-    if (a.splits > 1) {
-        const long long at = (((long long)split * a.batch + b) * a.heads + head) * a.q_len + i;
+    if (piece.split >= 0) {
+        const long long at = part_row(a.split, piece, wave * 32 + c32);
         if (half == 0) *(float2 *)(a.part_ml + 2 * at) = make_float2(m, l);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -273,12 +269,14 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttnFwdArgs a)
 template <int D>
 constexpr int kJoinLanes = D == 96 ? 32 : D / 4;               // (of 32 lanes 24 work for D = 96)
 template <int D, bool SHARED>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long long rows)
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a)
 {
     constexpr int CH = kJoinLanes<D>, G = SHARED ? 64 / CH : 1;
     const int lane = threadIdx.x & 63, g = SHARED ? lane / CH : 0, c = 4 * (lane % CH);
-    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / (CH * G);
+    const int at = (int)(blockIdx.x * 256 + threadIdx.x) / (CH * G), rows = a.split.part_rows();
     if (at >= rows) return;
+    const int item = a.split.whole + at / a.split.tile_rows, row = item % a.q_tiles * kBlockRows + at % a.split.tile_rows;
+    if (row >= a.rows) return;
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     auto merge = [&](float pm, float pl, f32x4 po) {
@@ -288,7 +286,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long
         l = l * f + pl * pf;
         o = o * f + po * pf;
     };
-    for (int s0 = g; s0 < a.splits; s0 += 4 * G) {
+    for (int s0 = g; s0 < a.split.splits; s0 += 4 * G) {
         float2 ml[4];
         f32x4 po[4];
 #pragma unroll
@@ -296,9 +294,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long
             const int s = s0 + k * G;
             ml[k] = make_float2(-INFINITY, 0.0f);
             po[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (s < a.splits) {
+            if (s < a.split.splits) {
                 ml[k] = *(const float2 *)(a.part_ml + 2 * (s * rows + at));
-                if (c < D) po[k] = *(const f32x4 *)(a.part_o + (s * rows + at) * D + c);
+                if (c < D) po[k] = *(const f32x4 *)(a.part_o + (long long)(s * rows + at) * D + c);
             }
         }
 #pragma unroll
@@ -312,19 +310,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnFwdArgs a, long
         for (int e = 0; e < 4; ++e) po[e] = __shfl_xor(o[e], d);
         merge(pm, pl, po);
     }
-    const int i = (int)(at % a.q_len);
-    const long long bh = at / a.q_len;
-    const int head = (int)(bh % a.heads);
+    const int gh = item / a.q_tiles % a.grid_heads, b = item / a.q_tiles / a.grid_heads, in_group = a.packed ? row / a.q_len : 0;
+    const int i = row - in_group * a.q_len, head = a.packed ? gh * a.group + in_group : gh;
+    const long long stat = ((long long)b * a.heads + head) * a.q_len + i;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (g == 0 && c < a.d) {
         bf16x4 w;
         o *= inv;
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = (__bf16)o[e];
-        if (a.o_exact) *(f32x4 *)(a.o_exact + at * a.d + c) = o;
-        *(bf16x4 *)(a.o + bh / a.heads * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
+        if (a.o_exact) *(f32x4 *)(a.o_exact + stat * a.d + c) = o;
+        *(bf16x4 *)(a.o + b * a.o_sb + (long long)i * a.o_st + head * a.o_sh + c) = w;
     }
-    if (a.lse && g == 0 && c == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
+    if (a.lse && g == 0 && c == 0) a.lse[stat] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
@@ -384,40 +382,56 @@ int check_result(const yamd_attention_desc *d, const yamd_tokens *t, int len, in
     return YAMD_OK;
 }
 
-// Parts that the looped axis of `tiles` tiles is split into.  From 512 workgroups on there is nothing to gain (800 workgroups
-// of 100 tiles, d 64: 276 us whole, 284 in two parts; 832 of 25: 97 and 125).  Below, the cost in units of a tile's time
-// is that of a CU with n workgroups, `resident` at a time and each `steps` tiles long (it takes up to three to hide the latency
-// of a tile, so fewer are no cheaper), plus the parts' way through memory and the launch that joins them (`tile`: a tile's
-// time against the forward kernel's).  The rule's numbers were fitted to six shapes of 24 to 208
-// workgroups: 300 queries on 8400 keys, 8 heads: 21 parts 18.4 us, 33 parts 21.3, whole 96; one query of 8 images: 22 parts
-// 17 us, 32 parts 20.9.
-int attention_splits(long long workgroups, int tiles, long long rows, int resident, float tile)
+// Costs are in units of a step's time on a CU with enough workgroups.  A CU works through its items one unit per step whether they
+// run side by side or one after the other, so what counts is the CU with the most.
+//
+// From 256 items on, what does not fill all 256 CUs is the loss (6400 keys, d 64: 768 items 208 us, 800 items 270 us, 1024 items
+// 280 us): as many items as fill them stay whole, and the rest is cut into parts that fill them once more.
+// Below, all items are cut.  The cost is that of a CU with n workgroups, `resident` at a time and each `steps` long (it takes up to
+// three to hide the latency of a step, so fewer are no cheaper).
+// Both pay for the parts' way through memory and for the launch that joins them.  The numbers were fitted to six shapes of 24 to
+// 208 items: 300 queries on 8400 keys, 8 heads: 21 parts 18.4 us, 33 parts 21.3, whole 96; one query of 8 images: 22 parts 17 us,
+// 32 parts 20.9.
+WorkSplit split_work(long long items, int steps, int len, int resident, int results, float step)
 {
-    if (workgroups >= 512) return 1;
-    const float per_part = (0.1f + (float)rows / 5000.0f) / tile, join = 12.0f / tile;
+    constexpr long long kCus = 256;
+    constexpr int kPrologue = 3;                         // steps that a part costs before its first and after its last one
+    const bool few = items < kCus;
+    const long long whole = few ? 0 : items / kCus * kCus, rest = items - whole;
+    const int tile_rows = len < kBlockRows ? len : kBlockRows;
+    const float rows = (float)(results * rest) * (float)len / (float)ceil_div(len, kBlockRows);
+    WorkSplit w = {(int)items, 0, 1, steps, tile_rows};
+    if (rest == 0) return w;
+    const float per_part = (0.1f + rows / 5000.0f) / step, join = 12.0f / step;
     const long long least = resident < 3 ? resident : 3;
-    int best = 1;
-    float best_cost = INFINITY;
-    for (int k = 1; k <= tiles && k <= 256;) {
-        const int steps = (tiles + k - 1) / k;
-        const long long n = (workgroups * k + 255) / 256, last = n % resident;
-        const long long load = n - last + (last == 0 ? 0 : last > least ? last : least);
-        const float cost = (float)steps * (float)load + (k > 1 ? per_part * (float)k + join : 0.0f);
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = k;
+    float best = INFINITY;
+    for (int k = 1; k <= 256;) {
+        const int len = (steps + k - 1) / k;
+        const long long n = (rest * k + kCus - 1) / kCus;
+        float cost;
+        if (few) {
+            const long long last = n % resident, load = n - last + (last == 0 ? 0 : last > least ? last : least);
+            cost = (float)len * (float)load;
+        } else {
+            cost = (float)(len + (k > 1 ? kPrologue : 0)) * (float)n;
         }
-        if (steps == 1) break;
-        k = (tiles + steps - 2) / (steps - 1);           // the next one with shorter parts: more parts of one length only cost more
+        if (k > 1) cost += per_part * (float)k + join;
+        if (cost < best) {
+            best = cost;
+            if (k > 1) w = {(int)whole, (int)rest, k, len, tile_rows};
+        }
+        if (len == 1) break;
+        k = (steps + len - 2) / (len - 1);               // the next one with shorter parts: more parts of one length only cost more
     }
-    return best;
+    w.splits = ceil_div(steps, w.per_split);
+    return w;
 }
 
 namespace {
 
 struct FwdPlan {
-    int packed, rows, q_tiles, grid_heads, splits, tiles_per_split, dpad;
-    long long total;
+    int packed, rows, q_tiles, grid_heads, dpad;
+    WorkSplit split;
     size_t workspace;
 };
 
@@ -431,40 +445,35 @@ FwdPlan plan_forward(const yamd_attention_desc *d, bool biased)
     p.rows = p.packed ? d->q_len * group : d->q_len;
     p.grid_heads = p.packed ? d->kv_heads : d->heads;
     p.q_tiles = ceil_div(p.rows, kBlockRows);
-    const int n_tiles = ceil_div(d->k_len, kTile);
-    const long long wgs = (long long)d->batch * p.grid_heads * p.q_tiles;
-    const int splits = attention_splits(wgs, n_tiles, (long long)d->batch * d->heads * d->q_len, p.dpad == 32 ? 4 : p.dpad == 64 ? 3 : 2, 1.0f);
-    p.tiles_per_split = ceil_div(n_tiles, splits);
-    p.splits = ceil_div(n_tiles, p.tiles_per_split);
-    p.total = wgs * p.splits;
-    if (p.splits > 1) p.workspace = (size_t)p.splits * d->batch * d->heads * d->q_len * (p.dpad + 2) * sizeof(float);
+    p.split = split_work((long long)d->batch * p.grid_heads * p.q_tiles, ceil_div(d->k_len, kTile), p.rows,
+                         p.dpad == 32 ? 4 : p.dpad == 64 ? 3 : 2, 1, 1.0f);
+    p.workspace = (size_t)p.split.splits * p.split.part_rows() * (p.dpad + 2) * sizeof(float);
     return p;
 }
 
 template <int D, int BIAS, bool EXACT>
-int launch_forward(const AttnFwdArgs &a, long long rows, hipStream_t st)
+int launch_forward(const AttnFwdArgs &a, hipStream_t st)
 {
     using Attr = KernelAttr<&attention_kernel<D, BIAS, EXACT>, FwdLds<D>::most(BIAS)>;
     const int lds = FwdLds<D>::WINDOW + 2 * a.window * (int)sizeof(float);
     const int rc = Attr::ensure();
     if (rc != YAMD_OK) return rc;
-    hipLaunchKernelGGL((attention_kernel<D, BIAS, EXACT>), dim3(work_grid(a.total)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attention_kernel<D, BIAS, EXACT>), dim3(a.split.grid()), dim3(256), lds, st, a);
     YAMD_LAUNCH_CHECK();
-    if (a.splits > 1) {
-        const long long lanes = rows * kJoinLanes<D>;
-        if (a.splits > 8) hipLaunchKernelGGL((attention_join_kernel<D, true>), dim3(ceil_div(rows * 64, 256)), dim3(256), 0, st, a, rows);
-        else hipLaunchKernelGGL((attention_join_kernel<D, false>), dim3(ceil_div(lanes, 256)), dim3(256), 0, st, a, rows);
+    if (const int rows = a.split.part_rows()) {
+        if (a.split.splits > 8) hipLaunchKernelGGL((attention_join_kernel<D, true>), dim3(ceil_div(rows * 64, 256)), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attention_join_kernel<D, false>), dim3(ceil_div(rows * kJoinLanes<D>, 256)), dim3(256), 0, st, a);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;
 }
 
 template <int D>
-int launch_forward(Bias form, const AttnFwdArgs &a, long long rows, hipStream_t st)
+int launch_forward(Bias form, const AttnFwdArgs &a, hipStream_t st)
 {
-    if (form == kNoBias) return launch_forward<D, kNoBias, false>(a, rows, st);
-    if (form == kQuadBias) return a.o_exact ? launch_forward<D, kQuadBias, true>(a, rows, st) : launch_forward<D, kQuadBias, false>(a, rows, st);
-    return a.o_exact ? launch_forward<D, kAnyBias, true>(a, rows, st) : launch_forward<D, kAnyBias, false>(a, rows, st);
+    if (form == kNoBias) return launch_forward<D, kNoBias, false>(a, st);
+    if (form == kQuadBias) return a.o_exact ? launch_forward<D, kQuadBias, true>(a, st) : launch_forward<D, kQuadBias, false>(a, st);
+    return a.o_exact ? launch_forward<D, kAnyBias, true>(a, st) : launch_forward<D, kAnyBias, false>(a, st);
 }
 
 }  // namespace
@@ -505,19 +514,15 @@ extern "C" int yamd_attention(const yamd_attention_desc *d, const yamd_tokens *q
         a.window = window_len(d->map_h, d->map_w);
     }
     a.batch = d->batch; a.q_len = d->q_len; a.k_len = d->k_len; a.d = d->head_dim; a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads;
-    a.packed = p.packed; a.rows = p.rows; a.q_tiles = p.q_tiles; a.grid_heads = p.grid_heads; a.splits = p.splits;
-    a.tiles_per_split = p.tiles_per_split; a.total = (int)p.total; a.scale = d->scale;
-    const long long rows = (long long)d->batch * d->heads * d->q_len;
-    if (p.splits > 1) {
-        a.part_o = (float *)workspace;
-        a.part_ml = a.part_o + (size_t)p.splits * rows * p.dpad;
-    }
+    a.packed = p.packed; a.rows = p.rows; a.q_tiles = p.q_tiles; a.grid_heads = p.grid_heads; a.split = p.split; a.scale = d->scale;
+    a.part_o = (float *)workspace;
+    if (p.workspace) a.part_ml = a.part_o + (size_t)p.split.splits * p.split.part_rows() * p.dpad;
     hipStream_t st = (hipStream_t)stream;
     const Bias form = bias_form(bias, d->map_h, d->map_w);
     switch (p.dpad) {
-    case 32: return launch_forward<32>(form, a, rows, st);
-    case 64: return launch_forward<64>(form, a, rows, st);
-    case 96: return launch_forward<96>(form, a, rows, st);
-    default: return launch_forward<128>(form, a, rows, st);
+    case 32: return launch_forward<32>(form, a, st);
+    case 64: return launch_forward<64>(form, a, st);
+    case 96: return launch_forward<96>(form, a, st);
+    default: return launch_forward<128>(form, a, st);
     }
 }

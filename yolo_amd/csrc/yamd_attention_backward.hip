@@ -27,17 +27,24 @@ struct AttnBwdArgs {
     int batch, q_len, k_len, d, heads, kv_heads, group;
     float scale;
     // one of the two owning kernels
-    int tiles, splits, loop_per_split, total;
+    int tiles;
+    WorkSplit split;
     __bf16 *out0, *out1;           // dk, dv / dq
     long long o0_sb, o0_st, o0_sh, o1_sb, o1_st, o1_sh;
-    float *part0, *part1;          // float32 parts [split][batch * heads][len][D] when splits > 1
-    float *part_bias;              // [batch * heads * tiles * splits][part_len]: sums by distance of one workgroup
-    int ring, part_len, window;
+    float *part0, *part1;          // results of parts: [part row][D]
+    float *part_bias;              // sums by distance of one workgroup: a row of whole_len for whole items, of part_len for parts
+    int ring, whole_len, part_len, window;
 };
 
 // the two rings of a wave lie 36 banks apart: the halves hold distances 4 apart, so that their 64 lanes meet 64 banks
 constexpr int kRingPad = 36;
 constexpr int kMostRing = 2048;                // positions for the widest map (w = 760: 2 * 128 + 8 + 2 * 128 + 2 w)
+
+// where the sums of a piece start
+__device__ __forceinline__ long long part_bias_at(const AttnBwdArgs &a, long long piece)
+{
+    return piece < a.split.whole ? piece * a.whole_len : (long long)a.split.whole * a.whole_len + (piece - a.split.whole) * a.part_len;
+}
 
 // D = rowsum(do o): 16 lanes per row, 8 channels each.  A row without keys (lse = -inf) has no gradient whatever do holds.
 // An error e of D adds -e P to a row's dS.  For dq, dk and dv that is far below the rounding of dS; the sums of a bias bucket
@@ -93,13 +100,11 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
     constexpr bool EARLY = D <= 64;                    // wider heads have no registers left to request operands ahead
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
-    int item = work_item();
-    if (item >= a.total) return;
-    const int split = item % a.splits;
-    item /= a.splits;
-    const int tile = item % a.tiles;
-    item /= a.tiles;
-    const int kv_head = item % a.kv_heads, b = item / a.kv_heads;
+    // the loop runs over (head of the group, tile of queries)
+    const int q_tiles = (a.q_len + ROWS - 1) / ROWS;
+    Piece piece;
+    if (!work_piece(a.split, a.group * q_tiles, piece)) return;
+    const int tile = piece.item % a.tiles, kv_head = piece.item / a.tiles % a.kv_heads, b = piece.item / a.tiles / a.kv_heads;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int key0 = tile * kBlockRows + wave * 32;
@@ -136,9 +141,7 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
     for (int n = 0; n < NB; ++n) dk[n] = zero16(), dv[n] = zero16();
     const float c2 = a.scale * kLog2e, inv_scale = 1.0f / a.scale;
 
-    // the loop runs over (head of the group, tile of queries)
-    const int q_tiles = (a.q_len + ROWS - 1) / ROWS, loop = a.group * q_tiles;
-    const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < loop ? t0 + a.loop_per_split : loop;
+    const int t0 = piece.t0, t1 = piece.t1;
     const TileLoader<D, ROWS> ql(a.q.st, a.d, wave, lane), gl(a.go.st, a.d, wave, lane);
     float lse_n = 0.0f, delta_n = 0.0f;
     auto fetch = [&](int t) {
@@ -256,8 +259,8 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
 #pragma unroll
         for (int n = 0; n < NB; ++n) dk[n] = zero16(), dv[n] = zero16();
     }
-    if (a.splits > 1) {
-        const long long at = ((((long long)split * a.batch + b) * a.kv_heads + kv_head) * a.k_len + key) * D;
+    if (piece.split >= 0) {
+        const long long at = (long long)part_row(a.split, piece, wave * 32 + c32) * D;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -316,7 +319,9 @@ template <int D>
 struct QLds {
     static constexpr int T = Tile<D>::bytes(kTile), BUF = 2 * T, COORD = 2 * BUF, KEEP = COORD + 2 * kTile * 4, WINDOW = KEEP + 16;
     static constexpr int most(bool biased) { return WINDOW + (biased ? 2 * 2048 * 4 + 8 * (kMostRing + kRingPad) * 4 : 0); }
-};template <int D, int BIAS>
+};
+
+template <int D, int BIAS>
 __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
 {
     using L = QLds<D>;
@@ -325,14 +330,10 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float *const rings = (float *)(smem + L::WINDOW) + 2 * a.window;
 
-    int item = work_item();
-    if (item >= a.total) return;
-    const int wg = item;
-    const int split = item % a.splits;
-    item /= a.splits;
-    const int tile = item % a.tiles;
-    item /= a.tiles;
-    const int head = item % a.heads, b = item / a.heads, kv_head = head / a.group;
+    Piece piece;
+    if (!work_piece(a.split, (a.k_len + kTile - 1) / kTile, piece)) return;
+    const int tile = piece.item % a.tiles, head = piece.item / a.tiles % a.heads, b = piece.item / a.tiles / a.heads, kv_head = head / a.group;
+    const int t0 = piece.t0, t1 = piece.t1;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
     const int row0 = tile * kBlockRows + wave * 32;
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         cq = a.coord_last + map_coord(row0 + c32, a.map_w);    // (lanes beyond the queries too have distances of their own)
         c_first = a.coord_last + map_coord(tile * kBlockRows, a.map_w);
         c_last = a.coord_last + map_coord(last, a.map_w);
-        high = c_last - map_coord(split * a.loop_per_split * kTile, a.map_w) + 1;      // distances from here on are written out
+        high = c_last - map_coord(t0 * kTile, a.map_w) + 1;                            // distances from here on are written out
         ring = rings + (2 * wave + half) * (a.ring + kRingPad);
         for (int e = tid; e < 8 * (a.ring + kRingPad); e += 256) rings[e] = 0.0f;
     }
@@ -380,8 +381,6 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     for (int n = 0; n < NB; ++n) dq[n] = zero16();
     const float c2 = a.scale * kLog2e;
 
-    const int n_tiles = (a.k_len + kTile - 1) / kTile;
-    const int t0 = split * a.loop_per_split, t1 = t0 + a.loop_per_split < n_tiles ? t0 + a.loop_per_split : n_tiles;
     auto window_from = [&](int t) { return c_first - map_coord(t * kTile + kTile - 1, a.map_w); };
     const TileLoader<D> kl(a.k.st, a.d, wave, lane), vl(a.v.st, a.d, wave, lane);
     unsigned char mask_n = 1;
@@ -398,7 +397,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     const int end_key = t1 * kTile < a.k_len ? t1 * kTile : a.k_len, coord_end = BIAS ? map_coord(end_key - 1, a.map_w) : 0;
     // writes the sums of the distances [low, high) out and clears them
     auto flush = [&](int low) {
-        float *out = a.part_bias + (long long)wg * a.part_len;
+        float *out = a.part_bias + part_bias_at(a, piece.index);
         const int base = c_first - coord_end;          // the smallest distance of the workgroup: first query, last key
         for (int e = low + tid; e < high; e += 256) {
             const int at = e & (a.ring - 1);
@@ -535,8 +534,8 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         flush(c_first - coord_end);
     }
     if (row0 + c32 >= a.q_len) return;
-    if (a.splits > 1) {
-        const long long at = ((((long long)split * a.batch + b) * a.heads + head) * a.q_len + i) * D;
+    if (piece.split >= 0) {
+        const long long at = (long long)part_row(a.split, piece, wave * 32 + c32) * D;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -560,21 +559,43 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         }
 }
 
-// Adds the workgroups' sums by distance: 64 distances x 16 threads per workgroup, thread y takes every 16th of a head's
-// (tile, split, image) triples and a tree in LDS adds the sixteen.
+// Adds the workgroups' sums by distance: 64 distances x 16 waves per workgroup, a wave takes every 16th of a head's (tile, image)
+// pairs and a tree in LDS adds the sixteen.  Which distances a piece has written follows from the coordinates of its rows and
+// keys; those need divisions, which would be most of the kernel if each pair made its own, so the lanes work them out for 64
+// tiles at a time (832 items of 40 x 40 tokens: 16 us, 23 us without).
 __global__ __launch_bounds__(1024) void attention_bias_grad_kernel(AttnBwdArgs a, float *dbias)
 {
     __shared__ float part[16][64];
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6, off = blockIdx.x * 64 + x, head = blockIdx.y;
+    const int x = threadIdx.x & 63, y = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), off = blockIdx.x * 64 + x, head = blockIdx.y;
+    const int per = a.split.per_split * kTile, step_t = 16 / a.batch, step_b = 16 % a.batch;
     float s = 0.0f;
-    for (int e = y; e < a.tiles * a.splits * a.batch; e += 16) {
-        const int b = e % a.batch, split = e / a.batch % a.splits, tile = e / a.batch / a.splits;
-        const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
-        const int end = (split + 1) * a.loop_per_split * kTile < a.k_len ? (split + 1) * a.loop_per_split * kTile : a.k_len;
-        const int base = a.coord_last + map_coord(tile * kBlockRows, a.map_w) - map_coord(end - 1, a.map_w);
-        const int top = a.coord_last + map_coord(last, a.map_w) - map_coord(split * a.loop_per_split * kTile, a.map_w);
-        if (off >= base && off <= top)
-            s += a.part_bias[((((long long)b * a.heads + head) * a.tiles + tile) * a.splits + split) * a.part_len + off - base];
+    auto add = [&](long long at, int base, int top) {
+        if (off >= base && off <= top) s += a.part_bias[at + off - base];
+    };
+    for (int t0 = 0; t0 < a.tiles; t0 += 64) {
+        const int row = (t0 + x < a.tiles ? t0 + x : a.tiles - 1) * kBlockRows;
+        const int first = a.coord_last + map_coord(row, a.map_w);
+        const int last = a.coord_last + map_coord(row + kBlockRows < a.q_len ? row + kBlockRows - 1 : a.q_len - 1, a.map_w);
+        const int n = a.tiles - t0 < 64 ? a.tiles - t0 : 64;
+        for (int t = y / a.batch, b = y % a.batch; t < n;) {
+            const int c_first = __builtin_amdgcn_readlane(first, t), c_last = __builtin_amdgcn_readlane(last, t);
+            const int item = (b * a.heads + head) * a.tiles + t0 + t;
+            if (item < a.split.whole) {
+                add((long long)item * a.whole_len, c_first - a.coord_last, c_last);
+            } else {
+                for (int k = 0; k < a.split.splits; ++k) {
+                    const int k0 = k * per, k1 = k0 + per < a.k_len ? k0 + per : a.k_len;
+                    add(part_bias_at(a, a.split.whole + (long long)(item - a.split.whole) * a.split.splits + k),
+                        c_first - map_coord(k1 - 1, a.map_w), c_last - map_coord(k0, a.map_w));
+                }
+            }
+            t += step_t;
+            b += step_b;
+            if (b >= a.batch) {
+                b -= a.batch;
+                ++t;
+            }
+        }
     }
     part[y][x] = s;
     __syncthreads();
@@ -587,11 +608,12 @@ __global__ __launch_bounds__(1024) void attention_bias_grad_kernel(AttnBwdArgs a
 }
 
 // Adds the parts of split results and rounds them; blockIdx.y picks one of up to three results, so that a backward pass needs
-// one launch for all of them (1447 tokens, 6 heads, d 64: 145 us instead of 152 with a launch each).
+// one launch for all of them (3 images of 1447 tokens, 6 heads, d 64, forward and
+// backward: 145 us instead of 152 with a launch each).
 struct SumOf {
     const float *parts;
-    long long rows;                // batch * heads * len
-    int splits, heads, len;
+    WorkSplit split;
+    int tiles, heads, len;
     float scale;
     __bf16 *out;
     long long sb, st, sh;
@@ -605,13 +627,13 @@ template <int D>
 __global__ __launch_bounds__(256) void attention_sum_parts_kernel(SumArgs args)
 {
     const SumOf a = args.of[blockIdx.y];
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, at = id / (D / 4);
-    const int c = (int)(id % (D / 4)) * 4;
-    if (at >= a.rows || c >= args.d) return;
+    const int id = blockIdx.x * 256 + threadIdx.x, at = id / (D / 4), c = id % (D / 4) * 4, rows = a.split.part_rows();
+    if (at >= rows || c >= args.d) return;
+    const int item = a.split.whole + at / a.split.tile_rows, t = item % a.tiles * kBlockRows + at % a.split.tile_rows;
+    if (t >= a.len) return;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < a.splits; ++k) s += *(const f32x4 *)(a.parts + (k * a.rows + at) * D + c);
-    const int t = (int)(at % a.len), head = (int)(at / a.len % a.heads);
-    const long long b = at / a.len / a.heads;
+    for (int k = 0; k < a.split.splits; ++k) s += *(const f32x4 *)(a.parts + (long long)(k * rows + at) * D + c);
+    const int head = item / a.tiles % a.heads, b = item / a.tiles / a.heads;
     bf16x4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = (__bf16)(s[e] * a.scale);
@@ -621,8 +643,8 @@ __global__ __launch_bounds__(256) void attention_sum_parts_kernel(SumArgs args)
 namespace {
 
 struct BwdPlan {
-    int dpad, kv_tiles, kv_splits, kv_loop, q_tiles, q_splits, q_loop, ring, part_len;
-    long long kv_total, q_total;
+    int dpad, kv_tiles, q_tiles, ring, whole_len, part_len;
+    WorkSplit kv, q;
     size_t delta, kv_parts, q_parts, bias, workspace;     // bytes
 };
 
@@ -636,25 +658,19 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     const int kt = ceil_div(d->k_len, kTile), qt = ceil_div(d->q_len, p.dpad <= 64 ? kTile : 32) * (d->heads / d->kv_heads);
     p.kv_tiles = ceil_div(d->k_len, kBlockRows);
     p.q_tiles = ceil_div(d->q_len, kBlockRows);
-    const long long kw = bk * p.kv_tiles, qw = bh * p.q_tiles;
-    const int ks = attention_splits(kw, qt, 2 * bk * d->k_len, p.dpad == 32 ? 4 : 2, 2.5f);
-    p.kv_loop = ceil_div(qt, ks);
-    p.kv_splits = ceil_div(qt, p.kv_loop);
-    const int qs = attention_splits(qw, kt, bh * d->q_len, p.dpad == 32 ? 3 : 2, 2.5f);
-    p.q_loop = ceil_div(kt, qs);
-    p.q_splits = ceil_div(kt, p.q_loop);
-    p.kv_total = kw * p.kv_splits;
-    p.q_total = qw * p.q_splits;
+    p.kv = split_work(bk * p.kv_tiles, qt, d->k_len, p.dpad == 32 ? 4 : 2, 2, 2.5f);
+    p.q = split_work(bh * p.q_tiles, kt, d->q_len, p.dpad == 32 ? 3 : 2, 1, 2.5f);
     p.delta = up256((size_t)bh * d->q_len * sizeof(float));
-    p.kv_parts = p.kv_splits > 1 ? up256(2 * (size_t)p.kv_splits * bk * d->k_len * p.dpad * sizeof(float)) : 0;
-    p.q_parts = p.q_splits > 1 ? up256((size_t)p.q_splits * bh * d->q_len * p.dpad * sizeof(float)) : 0;
+    p.kv_parts = up256(2 * (size_t)p.kv.splits * p.kv.part_rows() * p.dpad * sizeof(float));
+    p.q_parts = up256((size_t)p.q.splits * p.q.part_rows() * p.dpad * sizeof(float));
     if (biased) {
         const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + 8 + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
         for (p.ring = 256; p.ring < span; p.ring *= 2) {}
-        // distances of one workgroup: 128 queries against the keys of its part
-        const int keys = p.q_loop * kTile < d->k_len ? p.q_loop * kTile : d->k_len;
-        p.part_len = keys + kBlockRows + (d->map_h > 1 ? keys + kBlockRows + 2 * w : 0);
-        p.bias = up256((size_t)p.q_total * p.part_len * sizeof(float));
+        // distances of one workgroup: 128 queries against its keys
+        const auto distances = [&](int keys) { return keys + kBlockRows + (d->map_h > 1 ? keys + kBlockRows + 2 * w : 0); };
+        p.whole_len = distances(d->k_len);
+        p.part_len = distances(p.q.per_split * kTile < d->k_len ? p.q.per_split * kTile : d->k_len);
+        p.bias = up256(((size_t)p.q.whole * p.whole_len + (size_t)p.q.rest * p.q.splits * p.part_len) * sizeof(float));
     }
     p.workspace = p.delta + p.kv_parts + p.q_parts + p.bias;
     return p;
@@ -674,32 +690,31 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
     YAMD_LAUNCH_CHECK();
 
     AttnBwdArgs w = a;
-    w.tiles = p.kv_tiles; w.splits = p.kv_splits; w.loop_per_split = p.kv_loop; w.total = (int)p.kv_total;
+    w.tiles = p.kv_tiles; w.split = p.kv;
     w.out0 = (__bf16 *)dk->data; w.o0_sb = dk->batch_stride; w.o0_st = dk->token_stride; w.o0_sh = dk->head_stride;
     w.out1 = (__bf16 *)dv->data; w.o1_sb = dv->batch_stride; w.o1_st = dv->token_stride; w.o1_sh = dv->head_stride;
     w.part0 = a.delta + p.delta / sizeof(float);
-    w.part1 = w.part0 + (size_t)p.kv_splits * a.batch * a.kv_heads * a.k_len * D;
-    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256), KvLds<D>::WINDOW + 2 * a.window * (int)sizeof(float), st, w);
+    w.part1 = w.part0 + (size_t)p.kv.splits * p.kv.part_rows() * D;
+    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(w.split.grid()), dim3(256), KvLds<D>::WINDOW + 2 * a.window * (int)sizeof(float), st, w);
     YAMD_LAUNCH_CHECK();
     SumArgs sums = {};
     sums.d = a.d;
-    if (w.splits > 1) {
-        const long long r = (long long)a.batch * a.kv_heads * a.k_len;
-        sums.of[sums.n++] = {w.part0, r, w.splits, a.kv_heads, a.k_len, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh};
-        sums.of[sums.n++] = {w.part1, r, w.splits, a.kv_heads, a.k_len, 1.0f, w.out1, w.o1_sb, w.o1_st, w.o1_sh};
+    if (w.split.rest) {
+        sums.of[sums.n++] = {w.part0, w.split, w.tiles, a.kv_heads, a.k_len, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh};
+        sums.of[sums.n++] = {w.part1, w.split, w.tiles, a.kv_heads, a.k_len, 1.0f, w.out1, w.o1_sb, w.o1_st, w.o1_sh};
     }
 
     w = a;
-    w.tiles = p.q_tiles; w.splits = p.q_splits; w.loop_per_split = p.q_loop; w.total = (int)p.q_total;
+    w.tiles = p.q_tiles; w.split = p.q;
     w.out0 = (__bf16 *)dq->data; w.o0_sb = dq->batch_stride; w.o0_st = dq->token_stride; w.o0_sh = dq->head_stride;
     w.part0 = a.delta + (p.delta + p.kv_parts) / sizeof(float);
-    hipLaunchKernelGGL((attention_dq_kernel<D, BIAS>), dim3(work_grid(w.total)), dim3(256),
+    hipLaunchKernelGGL((attention_dq_kernel<D, BIAS>), dim3(w.split.grid()), dim3(256),
                        QLds<D>::WINDOW + (BIAS ? 2 * a.window + 8 * (p.ring + kRingPad) : 0) * (int)sizeof(float), st, w);
     YAMD_LAUNCH_CHECK();
-    if (w.splits > 1) sums.of[sums.n++] = {w.part0, rows, w.splits, a.heads, a.q_len, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh};
+    if (w.split.rest) sums.of[sums.n++] = {w.part0, w.split, w.tiles, a.heads, a.q_len, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh};
     if (sums.n) {
-        long long most = 0;
-        for (const SumOf &o : sums.of) most = o.rows > most ? o.rows : most;
+        int most = 0;
+        for (const SumOf &o : sums.of) most = o.split.part_rows() > most ? o.split.part_rows() : most;
         hipLaunchKernelGGL(attention_sum_parts_kernel<D>, dim3(ceil_div(most * (D / 4), 256), sums.n), dim3(256), 0, st, sums);
         YAMD_LAUNCH_CHECK();
     }
@@ -761,6 +776,7 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     a.part_bias = dbias ? (float *)((char *)workspace + p.delta + p.kv_parts + p.q_parts) : nullptr;
     a.o_exact = dbias ? o_exact : nullptr;
     a.ring = p.ring;
+    a.whole_len = p.whole_len;
     a.part_len = p.part_len;
     a.mask = key_mask; a.mask_sb = mask_stride; a.bias = bias;
     if (bias) {
