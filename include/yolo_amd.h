@@ -412,8 +412,8 @@ typedef struct yamd_attention_desc {
  *             key at (y', x') from [(y - y' + map_h - 1)(2 map_w - 1) + x - x' + map_w - 1].  Biases below -1e5 (-inf, the
  *             type's lowest value, ...) mask: a query with only such scores counts as left without keys (so with a bias the
  *             largest score of a query that has keys must lie above -1e5).
- *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted; only with a bias): o before its
- *             rounding to bf16 and with probabilities kept to 16 bits, which the gradient of a bias needs.
+ *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted): o before its rounding to
+ *             bf16, for the gradients; with a bias, or up to 256 keys, from probabilities kept to 16 bits.
  *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
  * Results must not overlap operands.  The workspace (16-byte aligned; may need no bytes) holds parts of o where the keys
  * are split over workgroups. */
@@ -421,8 +421,9 @@ size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biase
 int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
                    const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,
                    float *o_exact, float *lse, void *workspace, size_t workspace_bytes, void *stream);
-/* Gradients of the above from o, lse and d_o; the probabilities are computed again.  dbias: one float per head and distance
- * (NULL: the bias has no gradient; otherwise o_exact is needed too).  Every sum is taken in a fixed order: equal inputs give equal bits.
+/* Gradients of the above from o, lse and d_o; the probabilities are computed again.  o_exact may be NULL: gradients of
+ * queries with few keys or one dominant key are then up to several roundings of bf16 off.  dbias: one float per head and distance
+ * (NULL: the bias has no gradient; otherwise o_exact is needed).  Every sum is taken in a fixed order: equal inputs give equal bits.
  * Rows of o, dq, dk and dv must not overlap.  With a bias the workspace holds a row of sums by distance for every 128 queries of
  * a head, about q_len * k_len / 64 floats for a head of a map and half of that for a sequence. */
 size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *desc, int biased);

@@ -176,7 +176,7 @@ def test_attention_abi_refuses_bias_mask_workspace():
     assert _attention(_desc(map_h=10, map_w=11), bias=FAKE) == -1                # not q_len positions
     assert _attention(_desc(map_h=2, map_w=800, q_len=1600, k_len=1600), bias=FAKE) == -1
     assert _attention(_desc(), mask=FAKE, mask_stride=99) == -1
-    assert _attention(_desc(), exact=FAKE) == -1                                 # exact output without a bias
+    assert _attention(_desc(), exact=FAKE + 4) == -1
     big = _desc(batch=1, heads=1, kv_heads=1, q_len=1, k_len=100000)
     need = LIB.yamd_attention_workspace_bytes(ctypes.byref(big), 0)
     assert need > 0

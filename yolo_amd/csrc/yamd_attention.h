@@ -17,6 +17,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMasked = -1e5f;         // a query whose scores with their bias are all below this is left without keys
+constexpr int kFewKeys = 256;            // up to here o_exact takes two products without a bias too
 constexpr int kTile = 64;                // rows of a tile that passes through LDS (keys, or queries in the dK / dV kernel)
 constexpr int kBlockRows = 128;          // rows that a workgroup owns: 32 for each of its four waves
 

@@ -17,7 +17,7 @@ namespace yamd {
 
 struct AttnBwdArgs {
     AttnView q, k, v, o, go;
-    const float *o_exact;          // [batch][heads][q_len][d], in the place of o where the bias has a gradient
+    const float *o_exact;          // [batch][heads][q_len][d], in the place of o, or null
     const float *lse;
     float *delta;                  // [batch][heads][q_len]: D
     const uint8_t *mask;
@@ -47,9 +47,9 @@ __device__ __forceinline__ long long part_bias_at(const AttnBwdArgs &a, long lon
 }
 
 // D = rowsum(do o): 16 lanes per row, 8 channels each.  A row without keys (lse = -inf) has no gradient whatever do holds.
-// An error e of D adds -e P to a row's dS.  For dq, dk and dv that is far below the rounding of dS; the sums of a bias bucket
-// that holds most of a row's probability, where dS cancels, feel it in full (o rounded to bf16 left the table's gradient
-// 5e-3 off), so where the bias has a gradient o comes unrounded.
+// An error e of D adds -e P to a row's dS.  Where dS cancels that is felt: with o rounded to bf16 the gradient of a bias
+// bucket that holds most of a row's probability was 5e-3 off, dq of queries with 2 keys 5e-3 and with 20 keys 2.8e-3
+// (2.3e-3 is what the roundings of dS and of dq leave).  So o comes unrounded where the caller has it.
 __global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
 {
     const long long rows = (long long)a.batch * a.heads * a.q_len;
@@ -763,7 +763,8 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     if (rc != YAMD_OK) return rc;
     YAMD_REQUIRE(lse, "attention backward: lse is null");
     YAMD_REQUIRE(!dbias || bias, "attention backward: a bias gradient without a bias");
-    YAMD_REQUIRE(!dbias || (o_exact && ((uintptr_t)o_exact & 15) == 0), "attention backward: a bias gradient needs o_exact (16-byte aligned)");
+    YAMD_REQUIRE(!dbias || o_exact, "attention backward: a bias gradient needs o_exact");
+    YAMD_REQUIRE(((uintptr_t)o_exact & 15) == 0, "attention backward: o_exact is not 16-byte aligned");
     const BwdPlan p = plan_backward(d, bias != nullptr);
     if (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15)) {
         set_error("attention backward: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace ? workspace_bytes : (size_t)0, p.workspace);
@@ -774,7 +775,7 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     a.lse = lse;
     a.delta = (float *)workspace;
     a.part_bias = dbias ? (float *)((char *)workspace + p.delta + p.kv_parts + p.q_parts) : nullptr;
-    a.o_exact = dbias ? o_exact : nullptr;
+    a.o_exact = o_exact;
     a.ring = p.ring;
     a.whole_len = p.whole_len;
     a.part_len = p.part_len;

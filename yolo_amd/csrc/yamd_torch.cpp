@@ -259,7 +259,7 @@ AttentionOut attention_forward(const Tensor &q, const Tensor &k, const Tensor &v
         return r;
     }
     r.o = at::empty(q.sizes(), q.options());
-    if (stats && bias.defined() && bias.requires_grad())
+    if (stats)
         r.exact = at::empty({q.size(0), q.size(2), q.size(1), q.size(3)}, q.options().dtype(at::kFloat));
     const yamd_attention_desc d = descriptor(q, k, scale, h, w);
     const yamd_tokens tq = tokens(q), tk = tokens(k), tv = tokens(v), to = tokens(r.o);
