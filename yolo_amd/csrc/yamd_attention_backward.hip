@@ -52,38 +52,6 @@ __device__ __forceinline__ long long part_bias_at(const AttnBwdArgs &a, long lon
     return piece < a.split.whole ? piece * a.whole_len : (long long)a.split.whole * a.whole_len + (piece - a.split.whole) * a.part_len;
 }
 
-// D = rowsum(do o): 16 lanes per row, 8 channels each.  A row without keys (lse = -inf) has no gradient whatever do holds.
-// An error e of D adds -e P to a row's dS.  Where dS cancels that is felt: with o rounded to bf16 the gradient of a bias
-// bucket that holds most of a row's probability was 5e-3 off, dq of queries with 2 keys 5e-3 and with 20 keys 2.8e-3
-// (2.3e-3 is what the roundings of dS and of dq leave).  So o comes unrounded where the caller has it.
-__global__ __launch_bounds__(256) void attention_delta_kernel(AttnBwdArgs a)
-{
-    const long long rows = (long long)a.batch * a.heads * a.q_len;
-    const int c = (threadIdx.x & 15) * 8;
-    for (long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); at < rows; at += (long long)gridDim.x * 16) {
-        float s = 0.0f;
-        // rows in the order (batch, token, head), which is the order in memory of the usual layout
-        const int head = (int)(at % a.heads), i = (int)(at / a.heads % a.q_len);
-        const long long b = at / a.heads / a.q_len;
-        if (c < a.d) {
-            const bf16x8 g = *(const bf16x8 *)(a.go.p + b * a.go.sb + (long long)i * a.go.st + head * a.go.sh + c);
-            if (a.o_exact) {
-                const f32x4 *o = (const f32x4 *)(a.o_exact + ((b * a.heads + head) * a.q_len + i) * a.d + c);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s += o[e >> 2][e & 3] * (float)g[e];
-            } else {
-                const bf16x8 o = *(const bf16x8 *)(a.o.p + b * a.o.sb + (long long)i * a.o.st + head * a.o.sh + c);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s += (float)o[e] * (float)g[e];
-            }
-        }
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) s += __shfl_xor(s, d);
-        const long long w = (b * a.heads + head) * a.q_len + i;
-        if ((threadIdx.x & 15) == 0) a.delta[w] = a.lse[w] == -INFINITY ? 0.0f : s;
-    }
-}
-
 // ---- dk, dv ------------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys (the result's columns); tiles of 64 queries pass through LDS.  S = Q K^T and dP = dO V^T read the
 // tile's rows, dV^T += dO^T P and dK^T += Q^T dS read it transposed.
@@ -347,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     const long long stat = ((long long)b * a.heads + head) * a.q_len + i;
     const float lse = a.lse[stat];
     const bool valid = row0 + c32 < a.q_len && lse != -INFINITY;
-    const float lse2 = valid ? lse * kLog2e : INFINITY, delta = a.delta[stat];
+    const float lse2 = valid ? lse * kLog2e : INFINITY;
     const bool busy = __any(valid);
 
     bf16x8 qf[NKS], gf[NKS];
@@ -366,6 +334,31 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
             }
         }
     }
+    // D = rowsum(do o); a row without keys (lse = -inf) has no gradient whatever do holds.  An error e of D adds -e P to the row's
+    // dS.  Where dS cancels that is felt: with o rounded to bf16 the gradient of a bias bucket that holds most of a row's
+    // probability was 5e-3 off, dq of queries with 2 keys 4.9e-3 and with 20 keys 2.8e-3 (2.3e-3 is what the roundings of dS and
+    // of dq leave).  So o comes unrounded where the caller has it.
+    float delta = 0.0f;
+    if (valid) {
+        const float *ep = a.o_exact + stat * a.d;
+        const __bf16 *op = a.o.p + b * a.o.sb + (long long)i * a.o.st + head * a.o.sh;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            const int c = 16 * ks + 8 * half;
+            if (c >= a.d) continue;
+            if (a.o_exact) {
+                const f32x4 o0 = *(const f32x4 *)(ep + c), o1 = *(const f32x4 *)(ep + c + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) delta += o0[e] * (float)gf[ks][e] + o1[e] * (float)gf[ks][4 + e];
+            } else {
+                const bf16x8 o = *(const bf16x8 *)(op + c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta += (float)o[e] * (float)gf[ks][e];
+            }
+        }
+    }
+    delta = with_other_half(delta, [](float x, float y) { return x + y; });
+    if (half == 0 && row0 + c32 < a.q_len && piece.split <= 0) a.delta[stat] = delta;       // for the other kernel
     const __bf16 *kp = a.k.p + b * a.k.sb + kv_head * a.k.sh, *vp = a.v.p + b * a.v.sb + kv_head * a.v.sh;
     const uint8_t *mp = a.mask ? a.mask + b * a.mask_sb : nullptr;
 
@@ -691,33 +684,30 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
     int rc = KvAttr::ensure();
     if (rc == YAMD_OK) rc = QAttr::ensure();
     if (rc != YAMD_OK) return rc;
-    const long long rows = (long long)a.batch * a.heads * a.q_len;
-    hipLaunchKernelGGL(attention_delta_kernel, dim3(ceil_div(rows < (1 << 24) ? rows : 1 << 24, 16)), dim3(256), 0, st, a);
-    YAMD_LAUNCH_CHECK();
-
-    AttnBwdArgs w = a;
-    w.tiles = p.kv_tiles; w.split = p.kv;
-    w.out0 = (__bf16 *)dk->data; w.o0_sb = dk->batch_stride; w.o0_st = dk->token_stride; w.o0_sh = dk->head_stride;
-    w.out1 = (__bf16 *)dv->data; w.o1_sb = dv->batch_stride; w.o1_st = dv->token_stride; w.o1_sh = dv->head_stride;
-    w.part0 = a.delta + p.delta / sizeof(float);
-    w.part1 = w.part0 + (size_t)p.kv.splits * p.kv.part_rows() * D;
-    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(w.split.grid()), dim3(256), KvLds<D>::WINDOW + 2 * a.window * (int)sizeof(float), st, w);
-    YAMD_LAUNCH_CHECK();
     SumArgs sums = {};
     sums.d = a.d;
-    if (w.split.rest) {
-        sums.of[sums.n++] = {w.part0, w.split, w.tiles, a.kv_heads, a.k_len, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh};
-        sums.of[sums.n++] = {w.part1, w.split, w.tiles, a.kv_heads, a.k_len, 1.0f, w.out1, w.o1_sb, w.o1_st, w.o1_sh};
-    }
-
-    w = a;
-    w.tiles = p.q_tiles; w.split = p.q;
-    w.out0 = (__bf16 *)dq->data; w.o0_sb = dq->batch_stride; w.o0_st = dq->token_stride; w.o0_sh = dq->head_stride;
-    w.part0 = a.delta + (p.delta + p.kv_parts) / sizeof(float);
-    hipLaunchKernelGGL((attention_dq_kernel<D, BIAS>), dim3(w.split.grid()), dim3(256),
-                       QLds<D>::WINDOW + (BIAS ? 2 * a.window + 8 * (p.ring + kRingPad) : 0) * (int)sizeof(float), st, w);
+    // queries first: their kernel leaves D for the other one
+    AttnBwdArgs wq = a;
+    wq.tiles = p.q_tiles; wq.split = p.q;
+    wq.out0 = (__bf16 *)dq->data; wq.o0_sb = dq->batch_stride; wq.o0_st = dq->token_stride; wq.o0_sh = dq->head_stride;
+    wq.part0 = a.delta + (p.delta + p.kv_parts) / sizeof(float);
+    hipLaunchKernelGGL((attention_dq_kernel<D, BIAS>), dim3(wq.split.grid()), dim3(256),
+                       QLds<D>::WINDOW + (BIAS ? 2 * a.window + 8 * (p.ring + kRingPad) : 0) * (int)sizeof(float), st, wq);
     YAMD_LAUNCH_CHECK();
-    if (w.split.rest) sums.of[sums.n++] = {w.part0, w.split, w.tiles, a.heads, a.q_len, a.scale, w.out0, w.o0_sb, w.o0_st, w.o0_sh};
+    if (wq.split.rest) sums.of[sums.n++] = {wq.part0, wq.split, wq.tiles, a.heads, a.q_len, a.scale, wq.out0, wq.o0_sb, wq.o0_st, wq.o0_sh};
+
+    AttnBwdArgs wk = a;
+    wk.tiles = p.kv_tiles; wk.split = p.kv;
+    wk.out0 = (__bf16 *)dk->data; wk.o0_sb = dk->batch_stride; wk.o0_st = dk->token_stride; wk.o0_sh = dk->head_stride;
+    wk.out1 = (__bf16 *)dv->data; wk.o1_sb = dv->batch_stride; wk.o1_st = dv->token_stride; wk.o1_sh = dv->head_stride;
+    wk.part0 = a.delta + p.delta / sizeof(float);
+    wk.part1 = wk.part0 + (size_t)p.kv.splits * p.kv.part_rows() * D;
+    hipLaunchKernelGGL((attention_dkv_kernel<D, BIAS>), dim3(wk.split.grid()), dim3(256), KvLds<D>::WINDOW + 2 * a.window * (int)sizeof(float), st, wk);
+    YAMD_LAUNCH_CHECK();
+    if (wk.split.rest) {
+        sums.of[sums.n++] = {wk.part0, wk.split, wk.tiles, a.kv_heads, a.k_len, a.scale, wk.out0, wk.o0_sb, wk.o0_st, wk.o0_sh};
+        sums.of[sums.n++] = {wk.part1, wk.split, wk.tiles, a.kv_heads, a.k_len, 1.0f, wk.out1, wk.o1_sb, wk.o1_st, wk.o1_sh};
+    }
     if (sums.n) {
         int most = 0;
         for (const SumOf &o : sums.of) most = o.split.part_rows() > most ? o.split.part_rows() : most;
@@ -725,7 +715,7 @@ int launch_backward(AttnBwdArgs a, const BwdPlan &p, const yamd_tokens *dq, cons
         YAMD_LAUNCH_CHECK();
     }
     if (BIAS && dbias) {
-        hipLaunchKernelGGL(attention_bias_grad_kernel, dim3(ceil_div(a.n_off, 64), a.heads), dim3(1024), 0, st, w, dbias);
+        hipLaunchKernelGGL(attention_bias_grad_kernel, dim3(ceil_div(a.n_off, 64), a.heads), dim3(1024), 0, st, wq, dbias);
         YAMD_LAUNCH_CHECK();
     }
     return YAMD_OK;
