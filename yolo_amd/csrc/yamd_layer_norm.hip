@@ -9,8 +9,8 @@
 // that of the centred row, so a large mean costs no bits.  In the backward pass a thread adds dw and db of its channels
 // over its rows in registers, a workgroup adds its row groups in a fixed order and writes one partial row, and a second
 // kernel adds the partial rows in a fixed order: no atomics, the same bits on every run.
-// Measured: 51200 rows of 256 bf16 in 10 us (5.2 TB/s, what a copy reaches), 102400 rows of 512 with their gradients 94 us in
-// three launches for 420 MB (forward 35, backward 52, sums of the partial rows 7; 86 us at the rate of a copy).  Several rows are
+// Measured: 51200 rows of 256 bf16 in 10 us (5.2 TB/s, what a copy reaches), 102400 rows of 512 with their gradients 92 us in
+// three launches for 420 MB (forward 35, backward 52, sums of the partial rows 4; 86 us at the rate of a copy).  Several rows are
 // in flight per team because one row's loads do not cover the latency of memory (kRowsAtOnce).  Calls of a few hundred rows cost
 // their launches.
 // VEC > 1 (16-byte accesses) needs channel count, strides and addresses that are multiples of 16 bytes; other rows go
@@ -353,14 +353,24 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_backward_ker
     }
 }
 
-// column sums of the partial rows: 16 channels x 64 rows of threads per workgroup, blockIdx.y 0 = dw, 1 = db
+// column sums of the partial rows: 16 channels x 64 rows of threads per workgroup, blockIdx.y 0 = dw, 1 = db; a thread has
+// eight loads in flight
 __global__ __launch_bounds__(1024) void norm_param_grad_kernel(const float *partial, int n, int c, void *dw, void *db, int bf16)
 {
     __shared__ float lds[64][17];
     const int col = threadIdx.x & 15, row = threadIdx.x >> 4, ch = blockIdx.x * 16 + col;
     float s = 0.0f;
     if (ch < c)
-        for (int i = row; i < n; i += 64) s += partial[((long long)i * 2 + blockIdx.y) * c + ch];
+        for (int i0 = row; i0 < n; i0 += 8 * 64) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = i0 + 64 * k < n ? i0 + 64 * k : i0;
+                v[k] = partial[((long long)i * 2 + blockIdx.y) * c + ch];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += i0 + 64 * k < n ? v[k] : 0.0f;
+        }
     lds[row][col] = s;
     __syncthreads();
     for (int d = 32; d > 0; d >>= 1) {
