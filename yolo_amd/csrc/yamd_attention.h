@@ -259,6 +259,7 @@ __device__ __forceinline__ void load_window(char *lds, const float *bias, int fr
         load_lds_4(bias, (o < 0 ? 0 : o < n_off ? o : n_off - 1) * 4u, lds + at * 4);
     }
 }
+
 // Forms of the bias.  In quads (a sequence, or a map whose width is a multiple of 4) four tokens from a multiple of 4 on
 // lie next to each other, so one coordinate serves four rows of an accumulator.
 enum Bias { kNoBias, kAnyBias, kQuadBias };
@@ -281,11 +282,11 @@ __device__ __forceinline__ void read_bias(float (&b)[16], const float *win, cons
     }
 }
 
-// distances between 128 owned rows and a tile of 64, rounded up to what four waves load at once
 static inline Bias bias_form(const float *bias, int map_h, int map_w)
 {
     return !bias ? kNoBias : map_h == 1 || map_w % 4 == 0 ? kQuadBias : kAnyBias;
 }
+// distances between 128 owned rows and a tile of 64, rounded up to what four waves load at once
 static inline int window_len(int map_h, int map_w)
 {
     const int n = kBlockRows + kTile + (map_h > 1 ? kBlockRows + kTile + 2 * map_w : 0);
