@@ -44,6 +44,7 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Wall", "-Wno-
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HEADERS = [os.path.join(CSRC, "yamd_common.h"), os.path.join(CSRC, "yamd_conv_kernel.h"),
            os.path.join(CSRC, "yamd_conv_variants.inc"), os.path.join(CSRC, "yamd_attention.h"),
+           os.path.join(CSRC, "yamd_distance.h"),
            os.path.join(HERE, "..", "include", "yolo_amd.h")]
 
 

@@ -8,6 +8,7 @@
 // rows in their natural order: no probability ever moves between lanes.
 #pragma once
 #include "yamd_common.h"
+#include "yamd_distance.h"
 
 #include <cmath>
 
@@ -18,8 +19,6 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMasked = -1e5f;         // a query whose scores with their bias are all below this is left without keys
 constexpr int kFewKeys = 256;            // up to here o_exact takes two products without a bias too
-constexpr int kTile = 64;                // rows of a tile that passes through LDS (keys, or queries in the dK / dV kernel)
-constexpr int kBlockRows = 128;          // rows that a workgroup owns: 32 for each of its four waves
 
 struct AttnView {
     const __bf16 *p;
@@ -154,10 +153,6 @@ __device__ __forceinline__ int part_row(const WorkSplit &w, const Piece &p, int 
 {
     return (p.split * w.rest + p.item - w.whole) * w.tile_rows + row;
 }
-
-// A position t of a map of width w at (t / w, t % w) has the coordinate a(t) = (t / w)(2 w - 1) + t % w, and the distance of
-// two positions the index a(query) - a(key) + a(last) among the (2 h - 1)(2 w - 1) distances of the map.
-__host__ __device__ __forceinline__ int map_coord(int t, int w) { return t + (t / w) * (w - 1); }
 
 // Loads that write LDS directly: lane l of the wave takes 16 (4) bytes from `base` + `offset` and they land at byte 16 l
 // (4 l) behind `lds`; base and lds are the same for all lanes.  They are written as asm because the compiler, which cannot

@@ -269,10 +269,9 @@ __global__ __launch_bounds__(256, 2) void attention_dkv_kernel(AttnBwdArgs a)
 // The bias gradient is summed by distance.  For one key, the 32 queries of a half wave lie at 32 different distances, so
 // each half wave adds its dS values into a ring of float32 sums in LDS of its own without two lanes meeting: plain loads
 // and stores, in order within a wave.  (An LDS float atomic takes 81 ns per wave and CU, this 4 ns.)  As the
-// keys advance the distances fall: those above a(last query) - a(first key of the next tile) are final, and after each
-// tile the workgroup adds the eight rings in a fixed order for them, writes them to its row of the workspace and
-// clears them.  The ring must hold the distances of two tiles (one being added to while the other is written out):
-// 2 * 127 + 1 positions and the 4 below that quads touch, and where a map has several rows 127 + 127 + 2 w more.
+// keys advance the distances fall: those above a(last row) - a(first key of the next tile) are final (yamd_distance.h), and
+// after each tile the workgroup adds the eight rings in a fixed order for them, writes them to its row of the workspace and
+// clears them.
 // Four queries (lanes 4 i .. 4 i + 3) by four keys (accumulator rows r0 .. r0 + 3), both next to each other: lane 4 i + t
 // gets the sum of the diagonal that its own query makes with the first key (near), and of the one four distances below
 // (far; nothing for t = 0).  Half the additions to the ring are left.
@@ -362,15 +361,14 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
     const __bf16 *kp = a.k.p + b * a.k.sb + kv_head * a.k.sh, *vp = a.v.p + b * a.v.sb + kv_head * a.v.sh;
     const uint8_t *mp = a.mask ? a.mask + b * a.mask_sb : nullptr;
 
-    // distance index of (query, key) = cq - a(key); of the workgroup's rows the first and last
-    int cq = 0, c_first = 0, c_last = 0, high = 0;
+    // distance index of (query, key) = cq - a(key); of the workgroup's first row
+    int cq = 0, c_first = 0, high = 0;
     float *ring = nullptr;
+    auto final_at = [&](int t) { return final_from(tile, t * kTile, a.coord_last, a.map_w); };
     if constexpr (BIAS) {
-        const int last = tile * kBlockRows + kBlockRows - 1 < a.q_len ? tile * kBlockRows + kBlockRows - 1 : a.q_len - 1;
         cq = a.coord_last + map_coord(row0 + c32, a.map_w);    // (lanes beyond the queries too have distances of their own)
         c_first = a.coord_last + map_coord(tile * kBlockRows, a.map_w);
-        c_last = a.coord_last + map_coord(last, a.map_w);
-        high = c_last - map_coord(t0 * kTile, a.map_w) + 1;                            // distances from here on are written out
+        high = final_at(t0);                                   // distances from here on are written out
         ring = rings + (2 * wave + half) * (a.ring + kRingPad);
         for (int e = tid; e < 8 * (a.ring + kRingPad); e += 256) rings[e] = 0.0f;
     }
@@ -433,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void attention_dq_kernel(AttnBwdArgs a)
         if (mp) keep &= *kept;                         // (from LDS: all waves agree on the barrier below)
         keep = uniform64(keep);
         if (t + 1 < t1) fetch(t + 1);
-        if (BIAS && a.part_bias) flush(c_last - map_coord(t * kTile, a.map_w) + 1);   // what the tiles before this one left final
+        if (BIAS && a.part_bias) flush(final_at(t));   // what the tiles before this one left final
         if (keep == 0) continue;
         if (keep != ~0ull) {                           // a masked key may hold anything, NaN included
             clear_rows<D>(kt, keep);
@@ -663,12 +661,9 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
     p.kv_parts = up256(2 * (size_t)p.kv.splits * p.kv.part_rows() * p.dpad * sizeof(float));
     p.q_parts = up256((size_t)p.q.splits * p.q.part_rows() * p.dpad * sizeof(float));
     if (biased) {
-        const int w = d->map_h > 1 ? d->map_w : 1, span = 2 * kBlockRows + 8 + (d->map_h > 1 ? 2 * kBlockRows + 2 * w : 0);
-        for (p.ring = 256; p.ring < span; p.ring *= 2) {}
-        // distances of one workgroup: 128 queries against its keys
-        const auto distances = [&](int keys) { return keys + kBlockRows + (d->map_h > 1 ? keys + kBlockRows + 2 * w : 0); };
-        p.whole_len = distances(d->k_len);
-        p.part_len = distances(p.q.per_split * kTile < d->k_len ? p.q.per_split * kTile : d->k_len);
+        p.ring = ring_len(d->map_h, d->map_w);
+        p.whole_len = distances_of(d->k_len, d->map_h, d->map_w);
+        p.part_len = distances_of(p.q.per_split * kTile < d->k_len ? p.q.per_split * kTile : d->k_len, d->map_h, d->map_w);
         p.bias = up256(((size_t)p.q.whole * p.whole_len + (size_t)p.q.rest * p.q.splits * p.part_len) * sizeof(float));
     }
     p.workspace = p.delta + p.kv_parts + p.q_parts + p.bias;
