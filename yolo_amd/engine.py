@@ -463,7 +463,7 @@ class Program:
         d = q.c // heads
         if q.c != heads * d or k.c != kv_heads * d or v.c != k.c or (k.h, k.w) != (v.h, v.w) or heads % kv_heads:
             raise _lib.YamdError(f"attention[{name}]: {heads} heads over {q.c} channels do not fit {kv_heads} over {k.c} and {v.c}")
-        if not 8 <= d <= 128 or d % 8 or any(t.coff % 8 or self.buffers[t.buf][2] % 8 or self.buffers[t.buf][3] != torch.bfloat16 for t in (q, k, v)):
+        if not 8 <= d <= 128 or d % 8 or any(self.buffers[t.buf][3] != torch.bfloat16 for t in (q, k, v)):
             raise _lib.YamdError(f"attention[{name}]: heads must be 8 to 128 channels, a multiple of 8, of bf16 maps (got {d})")
         if (table is None) != (position is None):
             raise _lib.YamdError(f"attention[{name}]: table and position go together")
@@ -473,15 +473,25 @@ class Program:
         if out is None:
             out = self.buffer(q.h, q.w, q.c)
         assert (out.h, out.w, out.c) == (q.h, q.w, q.c), (name, out, q)
-        if self.buffers[out.buf][3] != torch.bfloat16 or out.coff % 8 or self.buffers[out.buf][2] % 8:
-            raise _lib.YamdError(f"attention[{name}]: the result must be a bf16 map whose channels start at a multiple of 8")
-        if any(t.buf == out.buf and t.coff < out.coff + out.c and out.coff < t.coff + t.c for t in (q, k, v)):
-            raise _lib.YamdError(f"attention[{name}]: the result overlaps an operand")
+        if self.buffers[out.buf][3] != torch.bfloat16:
+            raise _lib.YamdError(f"attention[{name}]: the result must be a bf16 map")
+        self._check_attention(name, q, k, v, out)
         layer = AttentionLayer(name, heads, kv_heads, d, (q.h, q.w), k.h * k.w, 1.0 / d ** 0.5 if scale is None else float(scale), table, position)
         layer.workspace = f"workspace {len(self.ops)} of {name}"
         self.stems.append(layer)
         self.ops.append(("attn", layer, q, k, v, out))
         return out
+
+    def _check_attention(self, name: str, q: View, k: View, v: View, out: View) -> None:
+        """Where the maps of an attention lie: called when it is recorded, and again when recording has ended, because ``cat`` can
+        move a buffer into a wider one later."""
+        at = [self.resolve(t) for t in (q, k, v, out)]
+        if any(coff % 8 or self.buffers[buf][2] % 8 for buf, coff in at):
+            raise _lib.YamdError(f"attention[{name}]: maps must start at a multiple of 8 channels, in buffers of a multiple of 8 channels "
+                                 "(also where a concatenation puts them)")
+        obuf, o0 = at[3]
+        if any(buf == obuf and c0 < o0 + out.c and o0 < c0 + t.c for t, (buf, c0) in zip((q, k, v), at)):
+            raise _lib.YamdError(f"attention[{name}]: the result overlaps an operand")
 
     def cat(self, views: List[View], name: Optional[str] = None) -> View:
         """torch.cat(views, dim=1) without moving data where possible: a source that is a whole buffer of its
@@ -906,6 +916,9 @@ class Program:
 
     def _buffers_for(self, batch: int, device) -> Dict[str, torch.Tensor]:
         if not self._finalized:
+            for op in self.ops:
+                if op[0] == "attn":
+                    self._check_attention(op[1].name, *op[2:])
             self._finalized = True
             if FUSE["upsample_cat"]:
                 self.fuse_upsample_cat()
