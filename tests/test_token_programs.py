@@ -46,3 +46,42 @@ def test_attention_maps_that_cat_moves_off_their_alignment():
     p, (q, k, v, wide) = _maps(64, 64, 64, 16)
     p.cat([wide, p.attention("a", q, k, v, 2)])
     p._buffers_for(1, "cpu")
+
+
+def _upsampled(write_between):
+    """low -> 2x -> cat with side -> 1x1 conv, with something written in between: over low, over the upsampled map, elsewhere."""
+    p = Program(64, 64)
+    low, side = p.buffer(8, 8, 64), p.buffer(16, 16, 64)
+    up = p.upsample2x(low)
+    write_between(p, low, up)
+    p.conv("reader", p.cat([up, side]), torch.zeros(64, 128, 1, 1), None, 1, L.ACT_NONE)
+    p._buffers_for(1, "cpu")
+    return [op[0] for op in p.ops]
+
+
+def test_upsampling_stays_where_its_source_is_normalised_in_place():
+    assert _upsampled(lambda p, low, up: None) == ["conv_cat2"]
+    assert _upsampled(lambda p, low, up: p.layer_norm("n", low, None, None)) == ["norm", "conv_cat2"]
+    assert _upsampled(lambda p, low, up: p.layer_norm("n", low, None, None, out=low)) == ["up2", "norm", "conv"]
+    qkv = lambda p: [p.buffer(8, 8, 64) for _ in range(3)]
+    assert _upsampled(lambda p, low, up: p.attention("a", *qkv(p), 1)) == ["attn", "conv_cat2"]
+    assert _upsampled(lambda p, low, up: p.attention("a", *qkv(p), 1, out=low)) == ["up2", "attn", "conv"]
+    wide = lambda p: [p.buffer(16, 16, 64) for _ in range(3)]
+    assert _upsampled(lambda p, low, up: p.attention("a", *wide(p), 1, out=up)) == ["up2", "attn", "conv"]
+
+
+def test_every_op_names_its_results():
+    p = Program(64, 64)
+    x = p.buffer(8, 8, 32)
+    y = p.conv("c", x, torch.zeros(32, 32, 1, 1), None, 1, L.ACT_NONE)
+    a, b = p.buffer(8, 8, 16), p.buffer(8, 8, 16)
+    p.conv("s", x, torch.zeros(32, 32, 1, 1), None, 1, L.ACT_NONE, out=a, out2=b)
+    u, m = p.upsample2x(x), p.maxpool2(x)
+    d = p.conv_transpose2x("t", x, torch.zeros(32, 32, 2, 2), None)
+    pools = p.buffer(8, 8, 96)
+    p.maxpool5_cascade(x, *(pools.slice(32 * i, 32) for i in range(3)))
+    n = p.layer_norm("n", x, None, None)
+    o = p.attention("o", x, y, n, 1)
+    got = [p._results_of(op) for op in p.ops]
+    t = p.ops[4][3]                                          # the 1x1 conv in front of the scatter
+    assert got == [[y], [a, b], [u], [m], [t], [d], [pools.slice(32 * i, 32) for i in range(3)], [n], [o]]

@@ -769,6 +769,23 @@ class Program:
             return list(op[2:5])
         return []
 
+    @staticmethod
+    def _results_of(op) -> List[View]:
+        kind = op[0]
+        if kind in ("focus", "nhwc16"):
+            return [op[1]]
+        if kind == "conv":
+            return [v for v in (op[3], op[5]) if v is not None]
+        if kind == "conv_cat2":
+            return [v for v in (op[6], op[7]) if v is not None]
+        if kind == "mp5":
+            return list(op[2:5])
+        if kind in ("bneck", "c3", "norm"):
+            return [op[3]]
+        if kind == "attn":
+            return [op[5]]
+        return [op[2]]                                      # stem, stem2, up2, copy, d2s, mp2
+
     def fuse_upsample_cat(self) -> int:
         """Removes every 2x upsampling whose output is one end of a concatenation that only 1x1 convs read: those convs
         then read the low-resolution tensor and the other part themselves (``conv_cat2`` ops), and neither the
@@ -802,6 +819,13 @@ class Program:
                     else:
                         readers.append((j, c0, c1))
             if not ok or not readers:
+                continue
+            # the readers take the low-resolution tensor later than the upsampling did: neither it nor the upsampled one must have
+            # been written again
+            lbuf, l0, l1 = rng(low)
+            between = self.ops[self.ops.index(up) + 1:max(j for j, _, _ in readers)]
+            if any(b == wb and c0 < w1 and c1 > w0 for op in between for b, c0, c1 in map(rng, self._results_of(op))
+                   for wb, w0, w1 in ((lbuf, l0, l1), (obuf, o0, o1))):
                 continue
             for j, c0, c1 in readers:
                 _, layer, x, y, _res, y2 = self.ops[j]
