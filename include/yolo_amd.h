@@ -379,7 +379,7 @@ int yamd_c3_fused(int cin, int ch, int cout, int act, const void *x, int x_cstri
 
 /* Layer norm over the c channels of each row (c <= 16384): y = (x - mean) / sqrt(var + eps) * weight + bias.
  * Rows of `dtype` x_stride elements apart; weight and bias (NULL = 1 and 0) of param_dtype.  mean and rstd (rows floats
- * each, both or neither) are what the backward pass needs.  y may be x.
+ * each, both or neither) are what the backward pass needs.  y may be x (with the same stride).
  * Backward: dx (NULL = not wanted) of dtype; dweight and dbias (NULL = not wanted) of param_dtype, c elements, the sums over
  * all rows; the workspace is needed for these two.  rows == 0 gives zero dweight and dbias. */
 int yamd_layer_norm(const void *x, long long x_stride, const void *weight, const void *bias, int param_dtype, float eps, void *y,

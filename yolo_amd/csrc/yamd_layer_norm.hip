@@ -470,6 +470,8 @@ extern "C" int yamd_layer_norm(const void *x, long long x_stride, const void *we
     YAMD_REQUIRE((mean == nullptr) == (rstd == nullptr), "layer norm: mean and rstd go together");
     YAMD_REQUIRE(eps >= 0.0f, "layer norm: eps must not be negative (got %g)", (double)eps);
     YAMD_REQUIRE(stride_ok(x_stride, c, rows) && stride_ok(y_stride, c, rows), "layer norm: row stride smaller than c=%d", c);
+    // (rows of different workgroups would meet)
+    YAMD_REQUIRE(x != y || rows <= 1 || x_stride == y_stride, "layer norm: in place with row strides %lld and %lld", x_stride, y_stride);
     NormArgs a = {};
     a.x = x; a.w = weight; a.b = bias; a.y = y; a.mean = mean; a.rstd = rstd;
     a.x_rs = x_stride; a.y_rs = y_stride; a.rows = rows; a.c = c; a.param_bf16 = param_dtype == YAMD_BF16; a.eps = eps;
