@@ -162,14 +162,20 @@ __device__ __forceinline__ unsigned lds_address(const void *p)
 {
     return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const __attribute__((address_space(3))) char *)p);
 }
+// (m0 is a register that the compiler keeps to itself: it warns about the declaration, and honours it)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds_16(const void *base, unsigned offset, const void *lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_address(lds)), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_address(lds)), "v"(offset), "s"(base)
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds_4(const void *base, unsigned offset, const void *lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_address(lds)), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_address(lds)), "v"(offset), "s"(base)
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Fills tiles with rows of a token axis of `len` rows (256 threads, each wave a quarter).  Rows beyond the axis repeat its
