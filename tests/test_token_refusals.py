@@ -31,3 +31,35 @@ def test_inline_assembly_declares_what_it_writes():
                 found += 1
                 assert '"m0"' in block.rsplit(":", 1)[1], (f, block)
     assert found >= 2
+
+
+def _calls():
+    """(operator over its floating-point arguments, those arguments)"""
+    x, w = torch.randn(4, 8), torch.ones(8)
+    q = torch.randn(1, 4, 1, 8).bfloat16()
+    pos = tokens.RelativePosition(2, 2, 8, 16, device="cpu")
+    table, bias = torch.zeros(pos.rows, 1), torch.zeros(1, pos.distances)
+    return [(lambda x, w, b: tokens.layer_norm(x, w, b), [x, w, w.clone()]),
+            (lambda q, k, v, b: tokens.attention(q, k, v, bias=b, position=pos), [q, q.clone(), q.clone(), bias]),
+            (lambda t: tokens.relative_bias(t, pos), [table])]
+
+
+def test_forward_mode_tangents_are_refused():
+    """(before anything else, so that a CPU tensor shows it; a tensor without a tangent gets to the next check)"""
+    with torch.autograd.forward_ad.dual_level():
+        for op, args in _calls():
+            for i in range(len(args)):
+                dual = list(args)
+                dual[i] = torch.autograd.forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(L.YamdError, match="forward-mode"):
+                    op(*dual)
+            with pytest.raises(L.YamdError, match="GPU"):
+                op(*args)
+
+
+def test_traces_are_refused():
+    for op, args in _calls():
+        with pytest.raises(L.YamdError, match="jit.trace"):
+            torch.jit.trace(op, tuple(args))
+        with pytest.raises(L.YamdError, match="GPU"):
+            op(*args)

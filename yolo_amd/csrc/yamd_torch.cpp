@@ -6,6 +6,7 @@
 // Results and workspaces come from torch's allocator on the current stream of the tensors' device, so calls on different
 // streams or inside different captured graphs share nothing.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -44,6 +45,15 @@ template <typename... A>
 void check(int rc, const char *what)
 {
     if (rc != YAMD_OK) fail(what, " failed (", rc, "): ", yamd_last_error());
+}
+
+// The kernels work on a tensor's memory alone: a forward-mode tangent would be dropped, and a trace would hold the result as a
+// constant.
+void refuse_tangents(const char *what, std::initializer_list<const Tensor *> tensors)
+{
+    if (at::tracer::impl::is_dispatch_enabled()) fail(what, " cannot be recorded by torch.jit.trace");
+    for (const Tensor *t : tensors)
+        if (t->defined() && t->_fw_grad(0).defined()) fail(what, " has no forward-mode derivative (an argument carries a tangent)");
 }
 
 void require_gpu(const Tensor &t, const char *name, const at::Device *device = nullptr)
@@ -153,6 +163,7 @@ struct LayerNorm : Function<LayerNorm> {
 Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, double eps)
 {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    refuse_tangents("layer_norm", {&x, &w, &b});
     require_gpu(x, "x");
     if (!known_dtype(x)) fail("x must be bfloat16 or float32, got ", x.scalar_type());
     if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > 16384) fail("x must have 1 to 16384 channels, got shape ", x.sizes());
@@ -207,6 +218,7 @@ struct RelativeBias : Function<RelativeBias> {
 
 Tensor relative_bias(const Tensor &table, const Tensor &bucket_of, const Tensor &order, const Tensor &start)
 {
+    refuse_tangents("relative_bias", {&table});
     const at::Device dev = bucket_of.device();
     const int64_t rows = start.numel() - 1;
     require_gpu(bucket_of, "position");
@@ -328,6 +340,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, std::optiona
                  const std::optional<Tensor> &bias_, int64_t h, int64_t w)
 {
     const Tensor mask = key_mask.value_or(Tensor()), bias = bias_.value_or(Tensor());
+    refuse_tangents("attention", {&q, &k, &v, &bias});
     require_gpu(q, "q");
     if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4)
         fail("q must be (batch, tokens, heads, channels) and k, v (batch, tokens, kv_heads, channels)");

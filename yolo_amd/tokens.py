@@ -2,7 +2,8 @@
 
 A map's NHWC pixels are its tokens: a (B, H, W, C) activation is ``(B, H*W, heads, C // heads)`` here without a copy, also as
 a channel slice of a wider buffer.  Tensors live on the GPU; attention takes bfloat16, layer norm bfloat16 or float32 rows.
-Gradients flow through ``torch.autograd`` (once: the gradients carry no graph of their own); all arithmetic happens inside
+Gradients flow through ``torch.autograd`` (once: the gradients carry no graph of their own; forward-mode tangents and
+``torch.jit.trace`` are refused); all arithmetic happens inside
 libyolo_amd.so, on torch's current stream of the tensors' device, and equal inputs give equal bits.  Results and scratch are
 torch allocations of each call, so calls on different streams, or captured into different graphs, share nothing.  A training
 step that is captured into a graph takes its forward and backward pass together; no eager result of the same leaves may be
