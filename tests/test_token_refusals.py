@@ -63,3 +63,17 @@ def test_traces_are_refused():
             torch.jit.trace(op, tuple(args))
         with pytest.raises(L.YamdError, match="GPU"):
             op(*args)
+
+
+def test_a_bias_without_gradient_needs_no_room_for_its_sums():
+    r = ctypes.byref
+    d = L.AttentionDesc(8, 8, 8, 64, 6400, 6400, 80, 80, 0.125)
+    size = LIB.yamd_attention_backward_workspace_bytes
+    plain, summed = size(r(d), 0), size(r(d), 1)
+    assert summed - plain > 8 * 8 * 6400 * 6400 // 64 * 4 * 0.9
+    t = L.Tokens(FAKE, 6400 * 512, 512, 64)
+    back = lambda dbias, nb: LIB.yamd_attention_backward(r(d), r(t), r(t), r(t), None, 0, FAKE, r(t), FAKE, FAKE, r(t), r(t), r(t), r(t), dbias,
+                                                         FAKE, nb, None)
+    # refused for want of room, with the room that is wanted in the message
+    assert back(None, plain - 1) == -3 and f"needs {plain} ".encode() in LIB.yamd_last_error()
+    assert back(FAKE, summed - 1) == -3 and f"needs {summed} ".encode() in LIB.yamd_last_error()

@@ -647,7 +647,8 @@ struct BwdPlan {
 
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
+// only a bias whose gradient is wanted has sums to keep
+BwdPlan plan_backward(const yamd_attention_desc *d, bool biased, bool bias_gradient)
 {
     BwdPlan p = {};
     p.dpad = padded_head_dim(d->head_dim);
@@ -664,7 +665,7 @@ BwdPlan plan_backward(const yamd_attention_desc *d, bool biased)
         p.ring = ring_len(d->map_h, d->map_w);
         p.whole_len = distances_of(d->k_len, d->map_h, d->map_w);
         p.part_len = distances_of(p.q.per_split * kTile < d->k_len ? p.q.per_split * kTile : d->k_len, d->map_h, d->map_w);
-        p.bias = up256(((size_t)p.q.whole * p.whole_len + (size_t)p.q.rest * p.q.splits * p.part_len) * sizeof(float));
+        if (bias_gradient) p.bias = up256(((size_t)p.q.whole * p.whole_len + (size_t)p.q.rest * p.q.splits * p.part_len) * sizeof(float));
     }
     p.workspace = p.delta + p.kv_parts + p.q_parts + p.bias;
     return p;
@@ -730,11 +731,11 @@ int launch_backward(Bias form, const AttnBwdArgs &a, const BwdPlan &p, const yam
 
 using namespace yamd;
 
-extern "C" size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *d, int biased)
+extern "C" size_t yamd_attention_backward_workspace_bytes(const yamd_attention_desc *d, int bias_gradient)
 {
     if (check_attention(d, nullptr, 0, nullptr) != YAMD_OK) return 0;
-    if (biased && (d->map_h <= 0 || d->map_w <= 0 || (long long)d->map_h * d->map_w != d->k_len)) return 0;
-    return plan_backward(d, biased != 0).workspace;
+    if (bias_gradient && (d->map_h <= 0 || d->map_w <= 0 || (long long)d->map_h * d->map_w != d->k_len)) return 0;
+    return plan_backward(d, bias_gradient != 0, bias_gradient != 0).workspace;
 }
 
 extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
@@ -756,7 +757,7 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     YAMD_REQUIRE(!dbias || bias, "attention backward: a bias gradient without a bias");
     YAMD_REQUIRE(!dbias || o_exact, "attention backward: a bias gradient needs o_exact");
     YAMD_REQUIRE(((uintptr_t)o_exact & 15) == 0, "attention backward: o_exact is not 16-byte aligned");
-    const BwdPlan p = plan_backward(d, bias != nullptr);
+    const BwdPlan p = plan_backward(d, bias != nullptr, dbias != nullptr);
     if (!workspace || workspace_bytes < p.workspace || ((uintptr_t)workspace & 15)) {
         set_error("attention backward: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace ? workspace_bytes : (size_t)0, p.workspace);
         return YAMD_ENOSPC;

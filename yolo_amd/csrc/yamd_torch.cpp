@@ -313,7 +313,7 @@ struct Attention : Function<Attention> {
                                                      ctx->saved_data["w"].toInt());
             const yamd_tokens tq = tokens(q), tk = tokens(k), tv = tokens(v), to = tokens(o), tg = tokens(go), tdq = tokens(dq), tdk = tokens(dk),
                               tdv = tokens(dv);
-            const size_t nbytes = yamd_attention_backward_workspace_bytes(&d, bias.defined());
+            const size_t nbytes = yamd_attention_backward_workspace_bytes(&d, dbias.defined());
             const Tensor ws = bytes(nbytes, q);
             check(yamd_attention_backward(&d, &tq, &tk, &tv, (const uint8_t *)ptr(mask), mask.defined() ? mask.stride(0) : 0,
                                           (const float *)ptr(bias), &to, (const float *)ptr(exact),
