@@ -421,8 +421,9 @@ size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biase
 int yamd_attention(const yamd_attention_desc *desc, const yamd_tokens *q, const yamd_tokens *k, const yamd_tokens *v,
                    const uint8_t *key_mask, long long mask_stride, const float *bias, const yamd_tokens *o,
                    float *o_exact, float *lse, void *workspace, size_t workspace_bytes, void *stream);
-/* Gradients of the above from o, lse and d_o; the probabilities are computed again.  o_exact may be NULL: gradients of
- * queries with few keys or one dominant key are then up to several roundings of bf16 off.  dbias: one float per head and distance
+/* Gradients of the above from o_exact, lse and d_o; the probabilities are computed again.  With o_exact o is not read and may be
+ * NULL.  o_exact may be NULL: D is then taken of o as it was rounded to bf16, and gradients of queries with few keys or one
+ * dominant key are up to several roundings of bf16 off.  dbias: one float per head and distance
  * (NULL: the bias has no gradient; otherwise o_exact is needed).  Every sum is taken in a fixed order: equal inputs give equal bits.
  * Rows of o, dq, dk and dv must not overlap.  With dbias (bias_gradient = 1) the workspace holds a row of sums by distance for every
  * 128 queries of a head, about q_len * k_len / 64 floats for a head of a map and half of that for a sequence: 0.2 GB for 8 images

@@ -25,3 +25,13 @@ def test_frozen_bias_gives_the_gradients_of_a_learned_one(gpu_device, h, w, head
     ref, tol = _reference(q, k, v, 1 / math.sqrt(d), mask, frozen, (h, w), do)
     for n, x in zip(("dq", "dk", "dv"), got):
         _within(n, x, ref[n], tol[n])
+
+
+def test_attention_result_may_change_before_its_backward_pass(gpu_device):
+    """The backward pass does not read o (it has the unrounded one)."""
+    leaves, do, _ = _inputs(gpu_device, 31, 2, 60, 90, 2, 1, 64)
+    want = torch.autograd.grad(tokens.attention(*leaves), leaves, do)
+    o = tokens.attention(*leaves)
+    o += 1.0
+    got = torch.autograd.grad(o, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

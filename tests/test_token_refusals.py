@@ -77,3 +77,14 @@ def test_a_bias_without_gradient_needs_no_room_for_its_sums():
     # refused for want of room, with the room that is wanted in the message
     assert back(None, plain - 1) == -3 and f"needs {plain} ".encode() in LIB.yamd_last_error()
     assert back(FAKE, summed - 1) == -3 and f"needs {summed} ".encode() in LIB.yamd_last_error()
+
+
+def test_attention_backward_takes_o_in_one_of_two_forms():
+    r = ctypes.byref
+    d = L.AttentionDesc(1, 2, 2, 64, 100, 100, 0, 0, 0.125)
+    t = L.Tokens(FAKE, 12800, 128, 64)
+    back = lambda o, exact: LIB.yamd_attention_backward(r(d), r(t), r(t), r(t), None, 0, None, o, exact, FAKE, r(t), r(t), r(t), r(t), None,
+                                                        None, 0, None)
+    odd = L.Tokens(FAKE + 2, 12800, 128, 64)
+    assert back(None, None) == -1 and back(r(odd), None) == -1 and back(r(odd), FAKE) == -1 and back(None, FAKE + 4) == -1
+    assert back(None, FAKE) == -3 and back(r(t), FAKE) == -3 and back(r(t), None) == -3          # all that is missing is the workspace

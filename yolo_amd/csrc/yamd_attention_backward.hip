@@ -747,7 +747,7 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
     if (rc == YAMD_OK) rc = check_tokens(d, q, d->q_len, d->heads, "q");
     if (rc == YAMD_OK) rc = check_tokens(d, k, d->k_len, d->kv_heads, "k");
     if (rc == YAMD_OK) rc = check_tokens(d, v, d->k_len, d->kv_heads, "v");
-    if (rc == YAMD_OK) rc = check_tokens(d, o, d->q_len, d->heads, "o");
+    if (rc == YAMD_OK && (o || !o_exact)) rc = check_tokens(d, o, d->q_len, d->heads, "o");
     if (rc == YAMD_OK) rc = check_tokens(d, d_o, d->q_len, d->heads, "do");
     if (rc == YAMD_OK) rc = check_result(d, dq, d->q_len, d->heads, "dq");
     if (rc == YAMD_OK) rc = check_result(d, dk, d->k_len, d->kv_heads, "dk");
@@ -763,7 +763,8 @@ extern "C" int yamd_attention_backward(const yamd_attention_desc *d, const yamd_
         return YAMD_ENOSPC;
     }
     AttnBwdArgs a = {};
-    a.q = view_of(q); a.k = view_of(k); a.v = view_of(v); a.o = view_of(o); a.go = view_of(d_o);
+    a.q = view_of(q); a.k = view_of(k); a.v = view_of(v); a.go = view_of(d_o);
+    if (o) a.o = view_of(o);
     a.lse = lse;
     a.delta = (float *)workspace;
     a.part_bias = dbias ? (float *)((char *)workspace + p.delta + p.kv_parts + p.q_parts) : nullptr;

@@ -290,7 +290,8 @@ struct Attention : Function<Attention> {
     {
         const Tensor bias = bias_.value_or(Tensor()), mask = mask_.value_or(Tensor());
         AttentionOut r = attention_forward(q, k, v, mask, bias, scale, h, w, true);
-        ctx->save_for_backward({q, k, v, bias, mask, r.o, r.lse, r.exact});
+        // (not o: the caller may change it)
+        ctx->save_for_backward({q, k, v, bias, mask, r.lse, r.exact});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["h"] = h;
         ctx->saved_data["w"] = w;
@@ -300,7 +301,7 @@ struct Attention : Function<Attention> {
     {
         once_only("attention");
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &v = s[2], &bias = s[3], &mask = s[4], &o = s[5], &lse = s[6], &exact = s[7];
+        const Tensor &q = s[0], &k = s[1], &v = s[2], &bias = s[3], &mask = s[4], &lse = s[5], &exact = s[6];
         const c10::DeviceGuard guard(q.device());
         const bool nothing = q.numel() == 0 || k.numel() == 0;
         auto result = [&](const Tensor &t) { return nothing ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options()); };
@@ -311,12 +312,11 @@ struct Attention : Function<Attention> {
             if (reinterpret_cast<uintptr_t>(go.data_ptr()) % 16) go = go.clone();      // (a piece of a longer vector)
             const yamd_attention_desc d = descriptor(q, k, ctx->saved_data["scale"].toDouble(), ctx->saved_data["h"].toInt(),
                                                      ctx->saved_data["w"].toInt());
-            const yamd_tokens tq = tokens(q), tk = tokens(k), tv = tokens(v), to = tokens(o), tg = tokens(go), tdq = tokens(dq), tdk = tokens(dk),
-                              tdv = tokens(dv);
+            const yamd_tokens tq = tokens(q), tk = tokens(k), tv = tokens(v), tg = tokens(go), tdq = tokens(dq), tdk = tokens(dk), tdv = tokens(dv);
             const size_t nbytes = yamd_attention_backward_workspace_bytes(&d, dbias.defined());
             const Tensor ws = bytes(nbytes, q);
             check(yamd_attention_backward(&d, &tq, &tk, &tv, (const uint8_t *)ptr(mask), mask.defined() ? mask.stride(0) : 0,
-                                          (const float *)ptr(bias), &to, (const float *)ptr(exact),
+                                          (const float *)ptr(bias), nullptr, (const float *)ptr(exact),
                                           (const float *)lse.data_ptr(), &tg, &tdq, &tdk, &tdv,
                                           (float *)ptr(dbias), ws.data_ptr(), nbytes, stream_of(q)),
                   "attention_backward");
