@@ -1,11 +1,15 @@
 """GPU tests of the token operators' less usual forms, against the 64-bit reference and bounds of test_gpu_tokens.py."""
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 
-from test_gpu_tokens import _check, _inputs, _reference, _within
+from test_gpu_tokens import _block, _block_inputs, _check, _index, _inputs, _reference, _within
+from yolo_amd import lib as L
 from yolo_amd import tokens
+from yolo_amd.engine import Program
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +39,105 @@ def test_attention_result_may_change_before_its_backward_pass(gpu_device):
     o += 1.0
     got = torch.autograd.grad(o, leaves, do)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("b,h,w,heads,kv,d", [
+    (2, 9, 12, 4, 2, 64), (1, 11, 13, 4, 1, 40), (1, 1, 333, 8, 2, 32), (2, 1, 50, 4, 2, 64), (1, 5, 7, 8, 4, 16), (1, 1, 1, 2, 1, 8),
+    (1, 20, 20, 4, 2, 128), (2, 7, 9, 6, 2, 96), (1, 1, 700, 4, 1, 104), (3, 8, 8, 2, 1, 120)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_bias_with_shared_key_heads(gpu_device, b, h, w, heads, kv, d, masked):
+    """dk and dv add over the heads of a group, each with its own bias."""
+    n = h * w
+    (q, k, v), do, g = _inputs(gpu_device, n + heads + d, b, n, n, heads, kv, d)
+    pos = tokens.RelativePosition(h, w, 8, 16, gpu_device)
+    table = torch.randn(pos.rows, heads, generator=g, device=gpu_device).requires_grad_()
+    mask = None
+    if masked:
+        mask = torch.rand(b, n, generator=g, device=gpu_device) < 0.6
+        mask[-1] = False
+    _check(gpu_device, q, k, v, do, mask=mask, table=table, pos=pos)
+
+
+@pytest.mark.parametrize("lq,lk,heads,kv,d,biased", [(70, 130, 4, 2, 64, False), (300, 2, 2, 2, 64, False), (33, 700, 2, 1, 96, False),
+                                                     (128, 64, 1, 1, 32, False), (1, 1, 1, 1, 8, False), (5, 3000, 4, 2, 128, False),
+                                                     (100, 100, 2, 1, 40, True)])
+def test_backward_from_the_rounded_result(gpu_device, lq, lk, heads, kv, d, biased):
+    """Through the C ABI without o_exact: D = rowsum(do o) takes over the rounding of o."""
+    b, scale = 2, 1 / math.sqrt(d)
+    leaves, do, g = _inputs(gpu_device, lq + lk + d, b, lq, lk, heads, kv, d)
+    q, k, v = (t.detach() for t in leaves)
+    bias = torch.randn(heads, 2 * lk - 1, generator=g, device=gpu_device) if biased else None
+    desc = L.AttentionDesc(b, heads, kv, d, lq, lk, int(biased), lk if biased else 0, scale)
+    r, tk = ctypes.byref, lambda t: ctypes.byref(L.Tokens(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)))
+    room = lambda n: torch.empty(max(n, 1), dtype=torch.uint8, device=gpu_device)
+    o, lse = torch.empty_like(q), torch.empty(b, heads, lq, device=gpu_device)
+    grads = [torch.full_like(t, math.nan) for t in (q, k, v)]
+    n = L.LIB.yamd_attention_workspace_bytes(r(desc), int(biased))
+    ws = room(n)
+    bp = None if bias is None else bias.data_ptr()
+    L.check(L.LIB.yamd_attention(r(desc), tk(q), tk(k), tk(v), None, 0, bp, tk(o), None, lse.data_ptr(), ws.data_ptr(), n, L.current_stream()))
+    n = L.LIB.yamd_attention_backward_workspace_bytes(r(desc), 0)
+    ws2 = room(n)
+    L.check(L.LIB.yamd_attention_backward(r(desc), tk(q), tk(k), tk(v), None, 0, bp, tk(o), None, lse.data_ptr(), tk(do),
+                                          *(tk(t) for t in grads), None, ws2.data_ptr(), n, L.current_stream()))
+    want, tol = _reference(q, k, v, scale, None, bias, (1, lk) if biased else None, do)
+    # the error of o reaches D, and dS by P times it: added to the bounds with the exact o
+    Q, G = q.double().transpose(1, 2), do.double().transpose(1, 2)
+    K = k.double().transpose(1, 2).repeat_interleave(heads // kv, 1)
+    s = scale * Q @ K.transpose(2, 3)
+    if biased:
+        s = s + bias.double()[:, _index(1, lk, gpu_device)]
+    p = torch.softmax(s, 3)
+    e_ds = 1.02 * p * (G.abs() * tol["o"].transpose(1, 2)).sum(3, keepdim=True)
+    fold = lambda t: t.reshape(b, kv, heads // kv, lk, d).sum(2)
+    tol["dq"] = tol["dq"] + (1.02 * scale * e_ds @ K.abs()).transpose(1, 2)
+    tol["dk"] = tol["dk"] + 1.02 * scale * fold(e_ds.transpose(2, 3) @ Q.abs()).transpose(1, 2)
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        _within(name, x, want[name], tol[name])
+    _within("o", o, want["o"], tol["o"])
+
+
+def test_two_host_threads_at_once(gpu_device):
+    """Two threads, each with its stream and its inputs, forward and backward: what one thread alone gets."""
+    cases = [_block_inputs(gpu_device, 60 + i, h=7 + 4 * i) for i in range(2)]
+
+    def step(leaves, pos, dy):
+        y = _block(*leaves, pos, 2)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, start = [[], []], threading.Barrier(2)
+
+    def work(i):
+        with torch.cuda.device(gpu_device), torch.cuda.stream(torch.cuda.Stream(gpu_device)):
+            start.wait()
+            for _ in range(20):
+                got[i].append(step(*cases[i]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for i in range(2):
+        assert len(got[i]) == 20
+        for one in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[i]))
+
+
+@pytest.mark.parametrize("c,first,n", [(64, 0, 64), (40, 0, 40), (24, 3, 17)])
+def test_program_normalises_in_place(gpu_device, c, first, n):
+    g = torch.Generator().manual_seed(c)
+    sd = dict(w=torch.randn(c, 3, 3, 3, generator=g), nw=torch.randn(n, generator=g), nb=torch.randn(n, generator=g))
+    out = []
+    for in_place in (False, True):
+        p = Program(32, 32)
+        x = p.conv("c", p.image16(), sd["w"], None, 2, L.ACT_NONE).slice(first, n)
+        y = x if in_place else p.buffer(x.h, x.w, c).slice(first, n)
+        p.outputs = {"y": p.layer_norm("n", x, sd["nw"], sd["nb"], out=y)}
+        for batch in (3, 1):
+            images = torch.rand(batch, 3, 32, 32, generator=torch.Generator().manual_seed(batch)).to(gpu_device)
+            out.append(p.run(images)["y"].clone())
+    assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[3])
