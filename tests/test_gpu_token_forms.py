@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_tokens import _block, _block_inputs, _check, _index, _inputs, _reference, _within
+from test_gpu_tokens import _block, _block_inputs, _check, _index, _inputs, _reference, _token_step, _within
 from yolo_amd import lib as L
 from yolo_amd import tokens
 from yolo_amd.engine import Program
@@ -141,3 +141,74 @@ def test_program_normalises_in_place(gpu_device, c, first, n):
             images = torch.rand(batch, 3, 32, 32, generator=torch.Generator().manual_seed(batch)).to(gpu_device)
             out.append(p.run(images)["y"].clone())
     assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[3])
+
+
+def _captured(step):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    return graph, out
+
+
+@pytest.mark.parametrize("which", ["layer_norm", "relative_bias", "attention", "attention over views"])
+def test_captured_backward_with_live_eager_results_is_refused(gpu_device, which):
+    """Each operator stops a captured backward pass before it reaches a leaf whose accumulator is an eager graph's on the default
+    stream; once the eager result is gone, the same step is captured and replays."""
+    (q, k, v), do, g = _inputs(gpu_device, 5, 1, 96, 96, 2, 2, 32)
+    pos = tokens.RelativePosition(8, 12, 8, 16, gpu_device)
+    n = lambda *s: torch.randn(*s, generator=g, device=gpu_device)
+    if which == "layer_norm":
+        leaves = [n(40, 64).bfloat16().requires_grad_(), n(64).requires_grad_(), n(64).requires_grad_()]
+        do, forward = n(40, 64).bfloat16(), lambda: tokens.layer_norm(*leaves)
+    elif which == "relative_bias":
+        leaves = [n(pos.rows, 2).requires_grad_()]
+        do, forward = n(2, pos.distances), lambda: tokens.relative_bias(leaves[0], pos)
+    elif which == "attention":
+        leaves, forward = [q, k, v], lambda: tokens.attention(q, k, v)
+    else:                                                    # (the leaf lies behind torch's own nodes)
+        leaves = [torch.stack((q, k, v), 2).detach().requires_grad_()]
+        forward = lambda: tokens.attention(*leaves[0].unbind(2))
+    step = lambda: torch.autograd.grad(forward(), leaves, do)
+    want = step()                                            # (its graph is gone when it returns)
+    alive = forward()
+    with pytest.raises(RuntimeError, match="eager result"):
+        _captured(step)
+    with torch.cuda.stream(torch.cuda.Stream(gpu_device)):   # without a capture nothing is refused
+        again = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    del alive
+    graph, out = _captured(step)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_captured_backward_refuses_through_a_whole_step(gpu_device):
+    pos = tokens.RelativePosition(8, 100, 8, 16, gpu_device)
+    n = lambda *s: torch.randn(*s, device=gpu_device)
+    leaves = [n(1, 800, 64).bfloat16().requires_grad_(), n(64).requires_grad_(), n(64).requires_grad_(), n(pos.rows, 2).requires_grad_()]
+    dy = n(1, 800, 2, 32).bfloat16()
+    alive = tokens.layer_norm(*leaves[:3])
+    with pytest.raises(RuntimeError, match="eager result"):
+        _captured(lambda: _token_step(leaves, pos, dy))
+    del alive
+    want = _token_step(leaves, pos, dy)
+    want = [t.detach() for t in want]
+    graph, out = _captured(lambda: [t.detach() for t in _token_step(leaves, pos, dy)])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_capture_asks_for_other_leaves_than_the_live_result(gpu_device):
+    """An eager result that holds only a leaf whose gradient the captured pass does not ask for is in nobody's way."""
+    (q, k, v), do, _ = _inputs(gpu_device, 6, 1, 50, 70, 2, 2, 32)
+    step = lambda: torch.autograd.grad(tokens.attention(q, k, v), (q,), do)
+    want = step()
+    alive = tokens.layer_norm(k)
+    graph, out = _captured(step)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0]) and alive.grad_fn is not None

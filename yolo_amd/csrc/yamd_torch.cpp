@@ -8,8 +8,11 @@
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -19,6 +22,8 @@
 #include <sstream>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/yolo_amd.h"
 
@@ -85,6 +90,40 @@ void once_only(const char *what)
     if (at::GradMode::is_enabled()) fail(what, " cannot be differentiated twice (create_graph=True)");
 }
 
+// A leaf has one accumulator for all live graphs that reach it, on the stream of the first.  If that was an eager graph on the
+// default stream, autograd would make the default stream wait for a captured one on the way there, which breaks the capture
+// and ends the process.  So a captured backward pass stops here when what it leads to holds a node of the default stream.
+void refuse_eager_nodes(const char *what, std::initializer_list<const Tensor *> inputs, c10::DeviceIndex device)
+{
+    using torch::autograd::Node;
+    const c10::hip::HIPStream none = c10::hip::getDefaultHIPStream(device);
+    if (c10::hip::getCurrentHIPStream(device) == none || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto *asked = torch::autograd::get_current_graph_task_exec_info();     // (empty: all that can be reached)
+    std::vector<Node *> todo;
+    std::unordered_set<Node *> seen;
+    auto visit = [&](Node *n) {
+        if (!n || !seen.insert(n).second) return;
+        if (asked && !asked->empty()) {
+            const auto it = asked->find(n);
+            if (it == asked->end() || !it->second.should_execute()) return;
+        }
+        todo.push_back(n);
+    };
+    for (const Tensor *t : inputs) {
+        if (!t->defined() || !t->requires_grad()) continue;
+        visit(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t).get() : t->grad_fn().get());
+        while (!todo.empty()) {
+            Node *n = todo.back();
+            todo.pop_back();
+            // (by id: autograd's streams and HIPStream name one device by two types)
+            const auto on = n->stream();
+            if (on && on->device_index() == device && on->id() == none.id())
+                fail(what, ": the backward pass is captured while an eager result of the same leaves is alive (delete it before the capture)");
+            for (const auto &e : n->next_edges()) visit(e.function.get());
+        }
+    }
+}
+
 // ---- layer norm ---------------------------------------------------------------------------------------------------------
 // row stride of (..., C) taken as evenly spaced rows
 int64_t row_stride(const Tensor &t, const char *name)
@@ -139,6 +178,7 @@ struct LayerNorm : Function<LayerNorm> {
         const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &mean = saved[3], &rstd = saved[4];
         const int64_t c = x.size(-1), n = x.numel() / c;
         const c10::DeviceGuard guard(x.device());
+        refuse_eager_nodes("layer_norm", {&x, &w, &b}, x.device().index());
         const Tensor dy = grads[0].contiguous();
         Tensor dx, dw, db, ws;
         if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
@@ -198,7 +238,7 @@ struct RelativeBias : Function<RelativeBias> {
     static Tensor forward(AutogradContext *ctx, const Tensor &table, const Tensor &bucket_of, const Tensor &order, const Tensor &start)
     {
         ctx->save_for_backward({order, start});
-        ctx->saved_data["dtype"] = (int64_t)table.scalar_type();
+        ctx->saved_data["table"] = table;
         return bias_forward(table, bucket_of);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -207,8 +247,10 @@ struct RelativeBias : Function<RelativeBias> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor d = grads[0].contiguous();
         const c10::DeviceGuard guard(d.device());
+        const Tensor table = ctx->saved_data["table"].toTensor();
+        refuse_eager_nodes("relative_bias", {&table}, d.device().index());
         const int64_t rows = saved[1].numel() - 1, heads = d.size(0);
-        Tensor dtable = at::empty({rows, heads}, d.options().dtype((at::ScalarType)ctx->saved_data["dtype"].toInt()));
+        Tensor dtable = at::empty({rows, heads}, d.options().dtype(table.scalar_type()));
         check(yamd_relative_bias_backward((const float *)d.data_ptr(), (const int32_t *)saved[0].data_ptr(), (const int32_t *)saved[1].data_ptr(),
                                           (int)d.size(1), (int)heads, (int)rows, dtable.data_ptr(), dtype_of(dtable), stream_of(d)),
               "relative_bias_backward");
@@ -303,6 +345,7 @@ struct Attention : Function<Attention> {
         const variable_list s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2], &bias = s[3], &mask = s[4], &lse = s[5], &exact = s[6];
         const c10::DeviceGuard guard(q.device());
+        refuse_eager_nodes("attention", {&q, &k, &v, &bias}, q.device().index());
         const bool nothing = q.numel() == 0 || k.numel() == 0;
         auto result = [&](const Tensor &t) { return nothing ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options()); };
         Tensor dq = result(q), dk = result(k), dv = result(v), dbias;

@@ -7,7 +7,8 @@ Gradients flow through ``torch.autograd`` (once: the gradients carry no graph of
 libyolo_amd.so, on torch's current stream of the tensors' device, and equal inputs give equal bits.  Results and scratch are
 torch allocations of each call, so calls on different streams, or captured into different graphs, share nothing.  A training
 step that is captured into a graph takes its forward and backward pass together; no eager result of the same leaves may be
-alive meanwhile (autograd would tie the captured stream to the eager one).
+alive meanwhile (autograd would tie the captured stream to the default one; where these operators' backward passes meet
+that, they raise before it breaks the capture).
 ``engine.Program`` records the forward passes into a layer program.
 """
 from typing import List, Optional
