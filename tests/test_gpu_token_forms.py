@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_tokens import _block, _block_inputs, _check, _index, _inputs, _reference, _token_step, _within
+from test_gpu_tokens import F, U, _block, _block_inputs, _check, _index, _inputs, _norm_case, _reference, _token_step, _within
 from yolo_amd import lib as L
 from yolo_amd import tokens
 from yolo_amd.engine import Program
@@ -212,3 +212,81 @@ def test_capture_asks_for_other_leaves_than_the_live_result(gpu_device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0], want[0]) and alive.grad_fn is not None
+
+
+@pytest.mark.parametrize("wanted", ["q", "k", "v", "bias", "qv", "k bias"])
+def test_gradients_of_some_arguments_only(gpu_device, wanted):
+    """The others need none: the same bits as when all do."""
+    h, w, heads = 7, 12, 2
+    (q, k, v), do, g = _inputs(gpu_device, 12, 2, h * w, h * w, heads, heads, 40)
+    pos = tokens.RelativePosition(h, w, 8, 16, gpu_device)
+    bias = tokens.relative_bias(torch.randn(pos.rows, heads, generator=g, device=gpu_device), pos).requires_grad_()
+    names = ["q", "k", "v", "bias"]
+    step = lambda leaves, asked: torch.autograd.grad(tokens.attention(*leaves[:3], bias=leaves[3], position=pos), asked, do)
+    want = dict(zip(names, step([q, k, v, bias], [q, k, v, bias])))
+    on = [n in (wanted.split() if " " in wanted or wanted == "bias" else wanted) for n in names]
+    leaves = [t.detach().clone().requires_grad_(x) for t, x in zip((q, k, v, bias), on)]
+    for n, got in zip([n for n, x in zip(names, on) if x], step(leaves, [t for t, x in zip(leaves, on) if x])):
+        assert torch.equal(got, want[n]), n
+
+
+def test_more_images_than_waves_share_a_bias(gpu_device):
+    """The sums by distance over 20 and 33 images: more than the 16 waves that take them in turns."""
+    for b in (20, 33):
+        (q, k, v), do, g = _inputs(gpu_device, b, b, 150, 150, 1, 1, 16)
+        pos = tokens.RelativePosition(10, 15, 8, 16, gpu_device)
+        table = torch.randn(pos.rows, 1, generator=g, device=gpu_device).requires_grad_()
+        _check(gpu_device, q, k, v, do, table=table, pos=pos)
+
+
+def test_very_many_small_images(gpu_device):
+    (q, k, v), do, _ = _inputs(gpu_device, 3, 70001, 1, 3, 2, 1, 16)
+    _check(gpu_device, q, k, v, do)
+
+
+def test_mask_rows_of_a_wider_mask(gpu_device):
+    (q, k, v), do, g = _inputs(gpu_device, 4, 3, 40, 70, 2, 2, 32)
+    wide = torch.rand(3, 100, generator=g, device=gpu_device) < 0.5
+    mask = wide[:, 7:77]
+    assert mask.data_ptr() % 4 and not mask.is_contiguous()
+    want = torch.autograd.grad(tokens.attention(q, k, v, None, mask.contiguous()), (q, k, v), do)
+    got = torch.autograd.grad(tokens.attention(q, k, v, None, mask), (q, k, v), do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_layer_norm_gradient_from_a_longer_vector(gpu_device):
+    """A gradient that starts off a 16-byte boundary takes the kernels of single channels: held to the bound."""
+    g = torch.Generator(device=gpu_device).manual_seed(8)
+    n = lambda *s: torch.randn(*s, generator=g, device=gpu_device)
+    for c in (64, 512, 1024, 8192):
+        x, w, b = n(70, c).requires_grad_(), n(c).requires_grad_(), n(c).requires_grad_()
+        dy = torch.cat([n(3), n(70 * c)])[3:].view(70, c)
+        assert dy.data_ptr() % 16 and dy.is_contiguous()
+        y = tokens.layer_norm(x, w, b)
+        want, tol = _norm_case(gpu_device, x, w, b, 1e-5, dy, F)
+        for name, a, r, t in zip(("dx", "dw", "db"), torch.autograd.grad(y, (x, w, b), dy), want[1:], tol[1:]):
+            _within(name, a, r, t + F * (r.abs() + t))
+
+
+@pytest.mark.parametrize("b,lq,lk,heads,kv,d,hw", [(2, 300, 8400, 2, 2, 32, None), (1, 1, 8400, 8, 2, 64, None), (1, 1600, 1600, 4, 2, 128, None),
+                                                   (1, 1447, 1447, 2, 2, 40, (1, 1447)), (1, 1600, 1600, 2, 2, 64, (40, 40)),
+                                                   (1, 1444, 1444, 2, 1, 104, (38, 38))])
+def test_long_axes_in_norm(gpu_device, b, lq, lk, heads, kv, d, hw):
+    """Elementwise bounds add worst cases over all keys.  Relative to the whole tensor a result carries two independent roundings to
+    bf16 (of P or dS, and its own), each at most U / sqrt(3) of it in the root mean square: twice that of both is allowed.  The
+    bias gradient takes float32 dS, whose error is that of D: one rounding's share."""
+    (q, k, v), do, g = _inputs(gpu_device, lq + lk + d, b, lq, lk, heads, kv, d)
+    bias, kw = None, {}
+    if hw:
+        pos = tokens.RelativePosition(*hw, 16, 40, gpu_device)
+        bias = tokens.relative_bias(torch.randn(pos.rows, heads, generator=g, device=gpu_device), pos).requires_grad_()
+        kw = dict(bias=bias, position=pos)
+    o = tokens.attention(q, k, v, **kw)
+    leaves = [q, k, v] + ([bias] if hw else [])
+    grads = torch.autograd.grad(o, leaves, do)
+    want, _ = _reference(q, k, v, 1 / math.sqrt(d), None, bias, hw, do)
+    rounding = U / math.sqrt(3)
+    for n, got in zip(("dq", "dk", "dv", "dbias", "o"), grads + (() if hw else (None,)) + (o,)):
+        if got is not None:
+            off = ((got.detach().double() - want[n]).norm() / want[n].norm()).item()
+            assert off <= (rounding if n == "dbias" else 2 * math.sqrt(2) * rounding), (n, off)
