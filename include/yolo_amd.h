@@ -415,6 +415,8 @@ typedef struct yamd_attention_desc {
  *   o_exact   (batch * heads * q_len * head_dim floats, 16-byte aligned; NULL = not wanted): o before its rounding to
  *             bf16, for the gradients; with a bias, or up to 256 keys, from probabilities kept to 16 bits.
  *   lse       (batch * heads * q_len floats; NULL = not wanted): log of the sum of exp of a query's scores, for backward.
+ * Scores are float32 and should stay below 1e6 in size: beyond, their rounding reaches the probabilities, and from 5e8 on a result may
+ * be NaN or zeros.
  * Results must not overlap operands.  The workspace (16-byte aligned; may need no bytes) holds parts of o where the keys
  * are split over workgroups. */
 size_t yamd_attention_workspace_bytes(const yamd_attention_desc *desc, int biased);

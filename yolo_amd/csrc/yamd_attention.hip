@@ -17,10 +17,10 @@
 // keys are split over workgroups whose float32 parts a second kernel joins.
 //
 // What bounds it: at d = 64 the vector unit (72 % busy, of which more than half are exponentials, quarter rate; matrix unit
-// 39 %): 2 images of 8 heads, 6400 x 6400 tokens take 225 us, 746 TFLOP/s; with a bias 300 us (78 %, the bias adds a load and
-// an addition per score).  At d = 128 nothing is full (vector 45 %, matrix 39 %, two waves per SIMD): 381 us, 880 TFLOP/s;
-// requesting operands ahead in a ring of registers did not help (386 us).  One query of 8 images on 8400 keys, d 64, moves
-// 69 MB in 18 us with the join.
+// 39 %): 2 images of 8 heads, 6400 x 6400 tokens take 210 us, 800 TFLOP/s; with a bias 256 us, and 338 us with the second
+// product (78 %, the bias adds a load and an addition per score).  At d = 128 nothing is full (vector 45 %, matrix 38 %, two waves per SIMD):
+// 375 - 385 us, 870 - 895 TFLOP/s; requesting operands ahead in a ring of registers did not help (386 us against 381 on one card).  One
+// query of 8 images on 8400 keys, d 64, moves 69 MB in 18 us with the join.
 #include "yamd_attention.h"
 
 #include <algorithm>

@@ -10,9 +10,9 @@
 // dS are rounded to bf16 there, their use in the sums before (bias) stays in float32.  Rounding dS costs dq and dk as much as
 // their own rounding (2.4e-3 instead of 1.7e-3 in all); a second product for what is lost took 12 % of the backward pass.
 //
-// What bounds them: neither unit is full, with two waves per SIMD.  2 images of 8 heads, 6400 x 6400 tokens, d = 64: dkv 376 us,
-// 892 TFLOP/s (matrix unit 41 % busy, vector unit 36 %), dq 270 us, 932 TFLOP/s (41 % and 49 %); d = 128 with 4 key heads: dkv
-// 716 us, 937 TFLOP/s (40 % and 27 %, LDS reads 10 %), dq 470 us, 1070 TFLOP/s (52 % and 39 %).  A third wave does not fit: the
+// What bounds them: neither unit is full, with two waves per SIMD.  2 images of 8 heads, 6400 x 6400 tokens, d = 64: dkv 373 us,
+// 900 TFLOP/s (matrix unit 41 % busy, vector unit 36 %), dq 269 us, 935 TFLOP/s (41 % and 48 %), with a bias 431 and 514 us; d = 128 with
+// 4 key heads: dkv 694 - 708 us, 950 TFLOP/s (40 % and 27 %, LDS reads 10 %), dq 446 - 469 us, 1070 - 1130 TFLOP/s (51 % and 38 %).  A third wave does not fit: the
 // results and the owned rows alone are 128 registers at d = 64, and asking for it spills.
 #include "yamd_attention.h"
 

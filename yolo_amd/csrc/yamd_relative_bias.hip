@@ -1,7 +1,7 @@
 // A learned position bias by buckets of distance: bias[head][distance] = table[bucket of the distance][head], and the
 // gradient of the table.  The attention kernels read the bias by distance ((2 h - 1)(2 w - 1) floats per head, for a 40 x 40
-// map 25 KB) and leave the sums of their score gradients by distance, so nothing of size tokens x tokens exists in either
-// direction.  Both kernels here move a few hundred kilobytes; a launch is what they cost.
+// map 25 KB) and leave the sums of their score gradients by distance, so no array of pairs exists in either
+// direction (the sums do take a row of distances for every 128 queries).  Both kernels here move a few hundred kilobytes; a launch is what they cost.
 // The gradient adds the distances of one bucket in a fixed order: threads stride over the bucket's list of distances
 // (sorted once, when the map of buckets is made) and a tree joins them.
 #include "yamd_common.h"

@@ -101,7 +101,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     position.distances) float32, see ``relative_bias``, for self-attention over the h x w map (or sequence) of ``position``;
     values below -1e5 (-inf, the type's lowest value, ...) mask, and a query with only such scores is left without keys
     (with a bias, the largest score of a query that has keys must lie above -1e5).
-    Scores, statistics and sums are float32; probabilities are rounded to bfloat16 for the products with v and do, and score
+    Scores, statistics and sums are float32 (scores should stay below 1e6 in size: beyond, their rounding reaches the
+    probabilities, and from 5e8 on a result may be NaN or zeros); probabilities are rounded to bfloat16 for the products with v and do, and score
     gradients for the products with q and k."""
     if (bias is None) != (position is None):
         raise _lib.YamdError("bias and position go together")
