@@ -290,3 +290,13 @@ def test_long_axes_in_norm(gpu_device, b, lq, lk, heads, kv, d, hw):
         if got is not None:
             off = ((got.detach().double() - want[n]).norm() / want[n].norm()).item()
             assert off <= (rounding if n == "dbias" else 2 * math.sqrt(2) * rounding), (n, off)
+
+
+@pytest.mark.parametrize("h,w,d", [(2, 760, 128), (3, 759, 40), (2, 760, 64), (1, 5001, 8), (600, 3, 96)])
+def test_widest_and_longest_maps(gpu_device, h, w, d):
+    """The most LDS that a bias takes, and distances far beyond a tile."""
+    n = h * w
+    (q, k, v), do, g = _inputs(gpu_device, n + d, 1, n, n, 1, 1, d)
+    pos = tokens.RelativePosition(h, w, 8, 64, gpu_device)
+    table = torch.randn(pos.rows, 1, generator=g, device=gpu_device).requires_grad_()
+    _check(gpu_device, q, k, v, do, table=table, pos=pos)
